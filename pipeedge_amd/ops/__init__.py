@@ -176,3 +176,76 @@ def embed_finish(x: Tensor, prefix: Tensor, pos: Tensor) -> Tensor:
     if _use_hip(x):
         return _hip.embed_finish(x, prefix, pos)
     return torch_ref.embed_finish(x, prefix, pos)
+
+
+def rotary_frequencies(rotary_dim: int, base: float = 10000.0,
+                       scaling: Optional[str] = None, factor: float = 1.0,
+                       original_length: Optional[int] = None,
+                       low_turns: float = 1.0, high_turns: float = 32.0,
+                       device=None) -> Tensor:
+    """Angle per position of each of ``rotary_dim / 2`` column pairs, float64.
+
+    Unscaled f_i = base^(-2i / rotary_dim). ``scaling`` stretches a model
+    trained for ``original_length`` positions to ``factor`` times as many:
+
+    - "linear": every f_i / factor;
+    - "base": base * factor^(rotary_dim / (rotary_dim - 2)) for base, which
+      keeps the first frequency and divides the last by ``factor``;
+    - "ramp": pairs that turn at least ``high_turns`` times within
+      ``original_length`` keep f_i, those below ``low_turns`` get
+      f_i / factor, between them the two are mixed linearly in the turns.
+    """
+    if rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError("rotary_frequencies: rotary_dim must be even, "
+                         f"got {rotary_dim}")
+    if not (base > 0.0 and factor > 0.0):
+        raise ValueError("rotary_frequencies: base and factor must be "
+                         "positive")
+    if scaling not in (None, "linear", "base", "ramp"):
+        raise ValueError(f"rotary_frequencies: unknown scaling: {scaling}")
+    if scaling == "base":
+        base = base * factor ** (rotary_dim / max(rotary_dim - 2, 1))
+    index = torch.arange(0, rotary_dim, 2, dtype=torch.float64)
+    freqs = base ** (-index / rotary_dim)
+    if scaling == "linear":
+        freqs = freqs / factor
+    elif scaling == "ramp":
+        if original_length is None or not high_turns > low_turns:
+            raise ValueError("rotary_frequencies: ramp needs original_length "
+                             "and high_turns > low_turns")
+        turns = original_length * freqs / (2.0 * math.pi)
+        keep = ((turns - low_turns) / (high_turns - low_turns)).clamp(0., 1.)
+        freqs = freqs * keep + freqs / factor * (1.0 - keep)
+    return freqs.to(device)
+
+
+def rotary(q: Tensor, positions: Tensor, freqs: Tensor,
+           k: Optional[Tensor] = None, *, interleaved: bool = False,
+           offset: int = 0, inverse: bool = False, scale: float = 1.0):
+    """Rotary positions of queries and, in the same launch, keys.
+
+    ``q`` is [.., heads, dim] and ``k`` the same but for its heads, in
+    bfloat16, float16 or float32 with any strides but 1 in the last
+    dimension; ``positions`` holds one integer a token ([..], any value) and
+    ``freqs`` the float64 vector of ``rotary_frequencies``. Columns
+    ``offset .. offset + 2 * len(freqs)`` of each head are turned, with the
+    pairs half that width apart or, ``interleaved``, next to each other; the
+    rest is copied. ``scale`` multiplies the turned columns. ``inverse`` turns
+    the other way, which is also the gradient. Returns new tensors: the turned
+    ``q``, or ``(q, k)``."""
+    run = _hip.rotary if _use_hip(q) else torch_ref.rotary
+    out = run(q, positions, freqs, k, interleaved, offset, inverse, scale,
+              False)
+    return out[0] if k is None else out
+
+
+def rotary_(q: Tensor, positions: Tensor, freqs: Tensor,
+            k: Optional[Tensor] = None, *, interleaved: bool = False,
+            offset: int = 0, inverse: bool = False, scale: float = 1.0):
+    """``rotary`` in place, for views of a larger tensor: the first 2H of the
+    3H heads of a packed qkv, the rotary columns of each head, rows of a
+    cache. ``q`` and ``k`` must not overlap. Returns its arguments."""
+    run = _hip.rotary if _use_hip(q) else torch_ref.rotary
+    out = run(q, positions, freqs, k, interleaved, offset, inverse, scale,
+              True)
+    return out[0] if k is None else out

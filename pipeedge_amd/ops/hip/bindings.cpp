@@ -33,6 +33,10 @@ std::vector<torch::Tensor> quant_encode_bf16(torch::Tensor x, int64_t bit,
 torch::Tensor quant_decode_bf16(torch::Tensor comm, torch::Tensor scale,
                                 torch::Tensor shift, int64_t bit,
                                 std::vector<int64_t> image_shape);
+std::tuple<torch::Tensor, c10::optional<torch::Tensor>> rotary_op(
+        torch::Tensor q, torch::Tensor positions, torch::Tensor freqs,
+        c10::optional<torch::Tensor> k, bool interleaved, int64_t offset,
+        bool inverse, double scale, bool in_place);
 
 namespace {
 
@@ -98,6 +102,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("quant_decode", &quant_decode_bf16, py::arg("comm"),
           py::arg("scale"), py::arg("shift"), py::arg("bit"),
           py::arg("image_shape"));
+    m.def("rotary", &rotary_op, py::arg("q"), py::arg("positions"),
+          py::arg("freqs"), py::arg("k") = py::none(),
+          py::arg("interleaved") = false, py::arg("offset") = 0,
+          py::arg("inverse") = false, py::arg("scale") = 1.0,
+          py::arg("in_place") = false);
     m.def("_debug_mfma_tile", &debug_mfma_tile);
     m.def("_debug_mfma32_raw", &debug_mfma32_raw);
     m.def("_debug_tr16_raw", &debug_tr16_raw);

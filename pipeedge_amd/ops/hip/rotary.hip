@@ -1,0 +1,343 @@
+// Rotary positions: each pair (a, b) of a head's columns is turned by the
+// angle position * frequency,
+//   a' = scale * (a cos - b sin),   b' = scale * (b cos + a sin),
+// with the pairs next to each other (interleaved) or half the rotated width
+// apart. The turn the other way (inverse) is also the gradient.
+//
+// The angle is formed and reduced in 64 bits from an fp64 frequency vector
+// instead of being read from a table: positions are then unbounded (a 32-bit
+// product is off by a whole turn near position 2^24), nothing can be indexed
+// out of range, and the trigonometry is paid once a token for all heads of
+// queries and keys, which share one launch. Bound by memory: every element
+// is read and written once, 16 B a lane.
+#include <torch/extension.h>
+
+#include <ATen/MemoryOverlap.h>
+#include <c10/core/DeviceGuard.h>
+
+#include "common.h"
+
+namespace {
+
+struct RotaryTensor {
+    const void* in;
+    void* out;
+    long in_b, in_s, in_h;      // strides in elements
+    long out_b, out_s, out_h;
+    int heads;
+};
+
+struct RotaryArgs {
+    RotaryTensor t[2];          // queries, keys (heads 0 = absent)
+    const void* positions;      // [B * S]
+    const double* freqs;        // [pairs]
+    int tokens, seq;            // B * S, S
+    int pairs, offset;          // rotated columns: offset .. offset + 2*pairs
+    int rot_items, items;       // work items a head, in all
+    int copy_lo;                // copied items below the rotated columns
+    int tokens_per_block;
+    unsigned items_magic;       // ceil(2^32 / items)
+    float scale, sign;
+};
+
+constexpr int ROTARY_THREADS = 256;
+
+template <typename T, int VEC> struct RotaryVec {
+    typedef T type __attribute__((ext_vector_type(VEC)));
+};
+template <typename T> struct RotaryVec<T, 1> { typedef T type; };
+
+template <typename T, int VEC>
+__device__ __forceinline__ void rotary_load(const T* p, float (&v)[VEC]) {
+    if constexpr (VEC == 1) {
+        v[0] = (float)p[0];
+    } else {
+        const auto x =
+            *reinterpret_cast<const typename RotaryVec<T, VEC>::type*>(p);
+        #pragma unroll
+        for (int j = 0; j < VEC; ++j) v[j] = (float)x[j];
+    }
+}
+
+template <typename T, int VEC>
+__device__ __forceinline__ void rotary_store(T* p, const float (&v)[VEC]) {
+    if constexpr (VEC == 1) {
+        p[0] = (T)v[0];
+    } else {
+        typename RotaryVec<T, VEC>::type x;
+        #pragma unroll
+        for (int j = 0; j < VEC; ++j) x[j] = (T)v[j];
+        *reinterpret_cast<typename RotaryVec<T, VEC>::type*>(p) = x;
+    }
+}
+
+// One block turns tokens_per_block tokens. An item is VEC pairs, or VEC
+// copied elements; a head has rot_items of the first and items - rot_items
+// of the second kind (none in place). VEC 1 serves any alignment.
+template <typename T, int VEC, bool INTERLEAVED, typename POS>
+__global__ __launch_bounds__(ROTARY_THREADS) void rotary_kernel(
+        RotaryArgs a) {
+    extern __shared__ float2 turns[];       // [tokens_per_block][pairs]
+    const int tok0 = blockIdx.x * a.tokens_per_block;
+    const int toks = min(a.tokens_per_block, a.tokens - tok0);
+
+    for (int i = threadIdx.x; i < toks * a.pairs; i += ROTARY_THREADS) {
+        const int t = i / a.pairs, p = i - t * a.pairs;
+        const double pos = (double)reinterpret_cast<const POS*>(
+            a.positions)[tok0 + t];
+        // in half turns, so that the reduction is exact; the remainder is
+        // in [-1, 1] and 32 bits are enough from there on
+        const double half_turns = pos * a.freqs[p] * 0.31830988618379067154;
+        const float rest = (float)(half_turns
+                                   - 2.0 * rint(half_turns * 0.5));
+        float s, c;
+        sincospif(rest, &s, &c);
+        turns[i] = make_float2(c * a.scale, s * a.scale * a.sign);
+    }
+    __syncthreads();
+
+    const int per_token = (a.t[0].heads + a.t[1].heads) * a.items;
+    int tok = 0, rest = threadIdx.x;
+    while (true) {
+        while (rest >= per_token) { rest -= per_token; ++tok; }
+        if (tok >= toks) break;
+        int head = (int)__umulhi((unsigned)rest, a.items_magic);
+        if (a.items == 1) head = rest;
+        const int item = rest - head * a.items;
+        const bool second = head >= a.t[0].heads;
+        const RotaryTensor& x = a.t[second ? 1 : 0];
+        if (second) head -= a.t[0].heads;
+        const int b = (tok0 + tok) / a.seq;
+        const int s = (tok0 + tok) - b * a.seq;
+        const T* in = reinterpret_cast<const T*>(x.in) + b * x.in_b
+                      + s * x.in_s + head * x.in_h;
+        T* out = reinterpret_cast<T*>(x.out) + b * x.out_b
+                 + s * x.out_s + head * x.out_h;
+        if (item < a.rot_items) {
+            const int p0 = item * VEC;
+            const float2* cs = turns + tok * a.pairs + p0;
+            float lo[VEC], hi[VEC];
+            if (INTERLEAVED) {
+                const T* p = in + a.offset + 2 * p0;
+                float even_odd[2][VEC];     // columns 2*p0 .. 2*p0+2*VEC
+                rotary_load<T, VEC>(p, even_odd[0]);
+                rotary_load<T, VEC>(p + VEC, even_odd[1]);
+                #pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    lo[j] = even_odd[(2 * j) / VEC][(2 * j) % VEC];
+                    hi[j] = even_odd[(2 * j + 1) / VEC][(2 * j + 1) % VEC];
+                }
+            } else {
+                rotary_load<T, VEC>(in + a.offset + p0, lo);
+                rotary_load<T, VEC>(in + a.offset + a.pairs + p0, hi);
+            }
+            #pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                const float2 t = cs[j];
+                const float x1 = lo[j] * t.x - hi[j] * t.y;
+                hi[j] = hi[j] * t.x + lo[j] * t.y;
+                lo[j] = x1;
+            }
+            if (INTERLEAVED) {
+                T* p = out + a.offset + 2 * p0;
+                float even_odd[2][VEC];
+                #pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    even_odd[(2 * j) / VEC][(2 * j) % VEC] = lo[j];
+                    even_odd[(2 * j + 1) / VEC][(2 * j + 1) % VEC] = hi[j];
+                }
+                rotary_store<T, VEC>(p, even_odd[0]);
+                rotary_store<T, VEC>(p + VEC, even_odd[1]);
+            } else {
+                rotary_store<T, VEC>(out + a.offset + p0, lo);
+                rotary_store<T, VEC>(out + a.offset + a.pairs + p0, hi);
+            }
+        } else {
+            int c = item - a.rot_items;
+            c = c < a.copy_lo ? c * VEC
+                              : c * VEC + 2 * a.pairs;
+            typedef typename RotaryVec<T, VEC>::type vec;
+            *reinterpret_cast<vec*>(out + c) =
+                *reinterpret_cast<const vec*>(in + c);
+        }
+        rest += ROTARY_THREADS;
+    }
+}
+
+// Whether all addresses of one tensor allow 16-byte accesses.
+bool rotary_aligned(const torch::Tensor& x, int vec) {
+    if (reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 != 0) return false;
+    for (int64_t d = 0; d + 1 < x.dim(); ++d)
+        if (x.size(d) > 1 && x.stride(d) % vec != 0) return false;
+    return true;
+}
+
+// [.., H, D] as [B, S, H, D] over the same memory
+torch::Tensor rotary_view4(const torch::Tensor& x, const char* name) {
+    TORCH_CHECK_VALUE(x.dim() >= 2, "rotary: ", name,
+                      " must be [.., heads, dim]");
+    TORCH_CHECK_VALUE(x.size(-1) <= 1 || x.stride(-1) == 1, "rotary: ", name,
+                      " must be contiguous in its last dimension");
+    if (x.dim() == 2) return x.unsqueeze(0).unsqueeze(0);
+    if (x.dim() == 3) return x.unsqueeze(0);
+    if (x.dim() == 4) return x;
+    auto sizes = x.sizes();
+    int64_t lead = 1;
+    for (int64_t d = 0; d + 3 < x.dim(); ++d) lead *= sizes[d];
+    return x.view({lead, sizes[x.dim() - 3], sizes[x.dim() - 2],
+                   sizes[x.dim() - 1]});
+}
+
+template <typename T, int VEC, bool INTERLEAVED>
+void rotary_launch(const RotaryArgs& a, bool wide, int blocks, size_t lds) {
+    if (wide)
+        hipLaunchKernelGGL((rotary_kernel<T, VEC, INTERLEAVED, int64_t>),
+                           dim3(blocks), dim3(ROTARY_THREADS), lds,
+                           pe_current_stream(), a);
+    else
+        hipLaunchKernelGGL((rotary_kernel<T, VEC, INTERLEAVED, int32_t>),
+                           dim3(blocks), dim3(ROTARY_THREADS), lds,
+                           pe_current_stream(), a);
+}
+
+template <typename T, int WIDE>
+void rotary_dispatch(const RotaryArgs& a, bool vec, bool interleaved,
+                     bool wide, int blocks, size_t lds) {
+    if (vec && interleaved) rotary_launch<T, WIDE, true>(a, wide, blocks, lds);
+    else if (vec) rotary_launch<T, WIDE, false>(a, wide, blocks, lds);
+    else if (interleaved) rotary_launch<T, 1, true>(a, wide, blocks, lds);
+    else rotary_launch<T, 1, false>(a, wide, blocks, lds);
+}
+
+}  // namespace
+
+std::tuple<torch::Tensor, c10::optional<torch::Tensor>> rotary_op(
+        torch::Tensor q, torch::Tensor positions, torch::Tensor freqs,
+        c10::optional<torch::Tensor> k, bool interleaved, int64_t offset,
+        bool inverse, double scale, bool in_place) {
+    TORCH_CHECK_VALUE(q.is_cuda(), "rotary: q must be a GPU tensor");
+    const c10::DeviceGuard guard(q.device());
+    const auto dtype = q.scalar_type();
+    TORCH_CHECK_TYPE(dtype == torch::kBFloat16 || dtype == torch::kHalf ||
+                     dtype == torch::kFloat,
+                     "rotary: q must be bfloat16, float16 or float32");
+    TORCH_CHECK_TYPE(positions.scalar_type() == torch::kInt ||
+                     positions.scalar_type() == torch::kLong,
+                     "rotary: positions must be int32 or int64");
+    TORCH_CHECK_TYPE(freqs.scalar_type() == torch::kDouble &&
+                     freqs.dim() == 1,
+                     "rotary: freqs must be a float64 vector");
+    TORCH_CHECK_VALUE(positions.device() == q.device() &&
+                      freqs.device() == q.device(),
+                      "rotary: tensors on different devices");
+    TORCH_CHECK_VALUE(!(at::GradMode::is_enabled() &&
+                        (q.requires_grad() ||
+                         (k.has_value() && k->requires_grad()))),
+                      "rotary: inference only, an input requires a gradient");
+    const int64_t pairs = freqs.numel(), dim = q.size(-1);
+    TORCH_CHECK_VALUE(pairs >= 1 && offset >= 0 && offset + 2 * pairs <= dim,
+                      "rotary: columns ", offset, " to ", offset + 2 * pairs,
+                      " do not fit a head of ", dim);
+    TORCH_CHECK_VALUE(pairs <= 1024, "rotary: more than 2048 rotated columns");
+    TORCH_CHECK_VALUE(positions.sizes() ==
+                      q.sizes().slice(0, std::max<int64_t>(q.dim() - 2, 0)),
+                      "rotary: positions must be one a token, shape ",
+                      q.sizes().slice(0, std::max<int64_t>(q.dim() - 2, 0)),
+                      ", got ", positions.sizes());
+    const auto q4 = rotary_view4(q, "q");
+    torch::Tensor k4;
+    if (k.has_value()) {
+        TORCH_CHECK_TYPE(k->scalar_type() == dtype,
+                         "rotary: q and k must have one type");
+        TORCH_CHECK_VALUE(k->device() == q.device(),
+                          "rotary: tensors on different devices");
+        TORCH_CHECK_VALUE(k->dim() == q.dim() && k->size(-1) == dim &&
+                          k->sizes().slice(0, q.dim() - 2) ==
+                          q.sizes().slice(0, q.dim() - 2),
+                          "rotary: k must match q except in its heads");
+        k4 = rotary_view4(*k, "k");
+    }
+    torch::Tensor q_out = q, k_out;
+    if (in_place) {
+        TORCH_CHECK_VALUE(at::has_internal_overlap(q) !=
+                          at::MemOverlap::Yes &&
+                          (!k.has_value() || at::has_internal_overlap(*k) !=
+                           at::MemOverlap::Yes),
+                          "rotary_: a tensor overlaps itself");
+        if (k.has_value()) {
+            const auto lap = at::get_overlap_status(q, *k);
+            TORCH_CHECK_VALUE(q.data_ptr() != k->data_ptr() &&
+                              lap != at::MemOverlapStatus::Full &&
+                              lap != at::MemOverlapStatus::Partial,
+                              "rotary_: q and k overlap");
+            k_out = *k;
+        }
+    } else {
+        q_out = torch::empty(q.sizes(), q.options());
+        if (k.has_value()) k_out = torch::empty(k->sizes(), k->options());
+    }
+    c10::optional<torch::Tensor> k_result;
+    if (k.has_value()) k_result = k_out;
+
+    const int64_t tokens = q4.size(0) * q4.size(1);
+    const int64_t heads = q4.size(2) + (k.has_value() ? k4.size(2) : 0);
+    if (tokens == 0 || heads == 0) return {q_out, k_result};
+    // the kernel's division by a reciprocal is exact below 2^32 / dim
+    TORCH_CHECK_VALUE(tokens < (1L << 31) && heads * dim * dim < (1L << 32),
+                      "rotary: too many tokens or columns");
+    const auto q4_out = in_place ? q4 : rotary_view4(q_out, "q");
+    const auto k4_out = !k.has_value() || in_place
+        ? k4 : rotary_view4(k_out, "k");
+
+    const int wide = dtype == torch::kFloat ? 4 : 8;
+    bool vec = pairs % wide == 0 && offset % wide == 0 && dim % wide == 0 &&
+        rotary_aligned(q4, wide) && rotary_aligned(q4_out, wide);
+    if (k.has_value())
+        vec = vec && rotary_aligned(k4, wide) && rotary_aligned(k4_out, wide);
+
+    RotaryArgs a = {};
+    const auto fill = [](RotaryTensor& t, const torch::Tensor& in,
+                         const torch::Tensor& out) {
+        t.in = in.data_ptr();
+        t.out = out.data_ptr();
+        t.in_b = in.stride(0), t.in_s = in.stride(1), t.in_h = in.stride(2);
+        t.out_b = out.stride(0), t.out_s = out.stride(1);
+        t.out_h = out.stride(2);
+        t.heads = in.size(2);
+    };
+    fill(a.t[0], q4, q4_out);
+    if (k.has_value()) fill(a.t[1], k4, k4_out);
+    const auto pos = positions.contiguous();
+    const auto freqs_c = freqs.contiguous();
+    a.positions = pos.data_ptr();
+    a.freqs = freqs_c.data_ptr<double>();
+    a.tokens = tokens;
+    a.seq = q4.size(1);
+    a.pairs = pairs;
+    a.offset = offset;
+    const int v = vec ? wide : 1;
+    a.rot_items = pairs / v;
+    a.copy_lo = offset / v;
+    a.items = a.rot_items + (in_place ? 0 : (dim - 2 * pairs) / v);
+    a.items_magic = (unsigned)(((1UL << 32) + a.items - 1) / a.items);
+    a.scale = scale;
+    a.sign = inverse ? -1.0f : 1.0f;
+    // three items a thread: enough blocks to fill the chip at a microbatch,
+    // and the trigonometry of a block is about one pair a thread
+    const long per_token = heads * a.items;
+    long tpb = (3 * ROTARY_THREADS + per_token - 1) / per_token;
+    tpb = std::min<long>(tpb, std::max<long>(1, 2048 / pairs));
+    a.tokens_per_block = std::min<long>(tpb, tokens);
+    const int blocks = (tokens + a.tokens_per_block - 1) / a.tokens_per_block;
+    const size_t lds = a.tokens_per_block * pairs * sizeof(float2);
+    const bool long_pos = pos.scalar_type() == torch::kLong;
+    if (dtype == torch::kBFloat16)
+        rotary_dispatch<__bf16, 8>(a, vec, interleaved, long_pos, blocks, lds);
+    else if (dtype == torch::kHalf)
+        rotary_dispatch<_Float16, 8>(a, vec, interleaved, long_pos, blocks,
+                                     lds);
+    else
+        rotary_dispatch<float, 4>(a, vec, interleaved, long_pos, blocks, lds);
+    HIP_CHECK_LAST();
+    return {q_out, k_result};
+}

@@ -13,7 +13,7 @@ k-contiguous per row, so A- and B-fragments alike stage through LDS with
 (cdna_hip_programming.md section 5).
 """
 import math
-from typing import Optional
+from typing import Optional, Tuple
 
 import torch
 from torch import Tensor
@@ -104,3 +104,80 @@ def patchify(pixels: Tensor, patch_size: int) -> Tensor:
     x = pixels.reshape(b, c, h // p, p, w // p, p)
     x = x.permute(0, 2, 4, 1, 3, 5)  # B, H/p, W/p, C, p, p
     return x.reshape(b, (h // p) * (w // p), c * p * p)
+
+
+def _check_inference(op: str, *tensors: Optional[Tensor]):
+    if torch.is_grad_enabled() and any(
+            t is not None and t.requires_grad for t in tensors):
+        raise ValueError(f"{op}: inference only, an input requires a gradient")
+
+
+def check_rotary(q: Tensor, positions: Tensor, freqs: Tensor,
+                 k: Optional[Tensor], offset: int, in_place: bool):
+    """The argument checks of the rotary kernel, for the CPU path."""
+    if q.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise TypeError("rotary: q must be bfloat16, float16 or float32")
+    if positions.dtype not in (torch.int32, torch.int64):
+        raise TypeError("rotary: positions must be int32 or int64")
+    if freqs.dtype != torch.float64 or freqs.dim() != 1:
+        raise TypeError("rotary: freqs must be a float64 vector")
+    if k is not None and k.dtype != q.dtype:
+        raise TypeError("rotary: q and k must have one type")
+    if any(t is not None and t.device != q.device
+           for t in (positions, freqs, k)):
+        raise ValueError("rotary: tensors on different devices")
+    _check_inference("rotary", q, k)
+    for name, x in (("q", q), ("k", k)):
+        if x is None:
+            continue
+        if x.dim() < 2:
+            raise ValueError(f"rotary: {name} must be [.., heads, dim]")
+        if x.shape[-1] > 1 and x.stride(-1) != 1:
+            raise ValueError(f"rotary: {name} must be contiguous in its "
+                             "last dimension")
+        if in_place and any(n > 1 and st == 0
+                            for n, st in zip(x.shape, x.stride())):
+            raise ValueError("rotary_: a tensor overlaps itself")
+    pairs, dim = freqs.numel(), q.shape[-1]
+    if pairs < 1 or offset < 0 or offset + 2 * pairs > dim:
+        raise ValueError(f"rotary: columns {offset} to {offset + 2 * pairs} "
+                         f"do not fit a head of {dim}")
+    if pairs > 1024:
+        raise ValueError("rotary: more than 2048 rotated columns")
+    if positions.shape != q.shape[:-2]:
+        raise ValueError("rotary: positions must be one a token, shape "
+                         f"{list(q.shape[:-2])}, got {list(positions.shape)}")
+    if k is not None:
+        if k.dim() != q.dim() or k.shape[-1] != dim \
+                or k.shape[:-2] != q.shape[:-2]:
+            raise ValueError("rotary: k must match q except in its heads")
+        if in_place and k.numel() and k.data_ptr() == q.data_ptr():
+            raise ValueError("rotary_: q and k overlap")
+
+
+def rotary(q: Tensor, positions: Tensor, freqs: Tensor,
+           k: Optional[Tensor] = None, interleaved: bool = False,
+           offset: int = 0, inverse: bool = False, scale: float = 1.0,
+           in_place: bool = False) -> Tuple[Tensor, Optional[Tensor]]:
+    """Turn column pairs by ``position * freqs`` (angles in 64 bits)."""
+    check_rotary(q, positions, freqs, k, offset, in_place)
+    angle = positions.to(torch.float64).unsqueeze(-1) * freqs
+    if inverse:
+        angle = -angle
+    cos = (torch.cos(angle) * scale).float().unsqueeze(-2)
+    sin = (torch.sin(angle) * scale).float().unsqueeze(-2)
+    width = 2 * freqs.numel()
+
+    def _turn(x):
+        part = x[..., offset:offset + width].float()
+        a, b = (part[..., 0::2], part[..., 1::2]) if interleaved \
+            else part.chunk(2, dim=-1)
+        turned = (a * cos - b * sin, b * cos + a * sin)
+        turned = torch.stack(turned, dim=-1).flatten(-2) if interleaved \
+            else torch.cat(turned, dim=-1)
+        out = x if in_place else x.clone(
+            memory_format=torch.contiguous_format)
+        out[..., offset:offset + width] = turned.to(x.dtype)
+        return out
+
+    return _turn(q), None if k is None else _turn(k)
