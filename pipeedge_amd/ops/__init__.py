@@ -249,3 +249,28 @@ def rotary_(q: Tensor, positions: Tensor, freqs: Tensor,
     out = run(q, positions, freqs, k, interleaved, offset, inverse, scale,
               True)
     return out[0] if k is None else out
+
+
+def latent_attention(q: Tensor, kv: Tensor, k_rope: Tensor, *,
+                     scale: Optional[float] = None, causal: bool = False,
+                     lengths: Optional[Tensor] = None,
+                     past: Optional[Tensor] = None) -> Tensor:
+    """Attention over latent vectors in expanded form, for prompts.
+
+    ``q`` [B, Sq, H, DN + DR] holds plain and rotated columns, ``kv``
+    [B, Sk, H, 2 DN] the keys' plain columns and the values of each head (the
+    latent vectors' up-projection, as ``linear`` writes it) and ``k_rope``
+    [B, Sk, DR] the rotated key columns that all heads share; DN is 64 or 128,
+    DR 32 or 64, all bfloat16 or float16 (any strides). Returns [B, Sq, H, DN];
+    ``scale`` is 1 / sqrt(DN + DR) unless given.
+
+    ``lengths`` (int32 [B]) are the valid keys of each padded sequence, ``past``
+    (int32 [B]) the position of its first query, Sk - Sq if both are absent; a
+    ``causal`` query sees no key behind its own position. Queries whose
+    position is outside their sequence are padding and come back zero; keys
+    and values behind a sequence may hold anything. A non-finite value inside
+    a sequence also reaches the earlier queries of its tile."""
+    if scale is None:
+        scale = 1.0 / math.sqrt(max(q.shape[-1], 1))
+    run = _hip.latent_attention if _use_hip(q) else torch_ref.latent_attention
+    return run(q, kv, k_rope, scale, causal, lengths, past)

@@ -37,6 +37,10 @@ std::tuple<torch::Tensor, c10::optional<torch::Tensor>> rotary_op(
         torch::Tensor q, torch::Tensor positions, torch::Tensor freqs,
         c10::optional<torch::Tensor> k, bool interleaved, int64_t offset,
         bool inverse, double scale, bool in_place);
+torch::Tensor latent_attention_op(
+        torch::Tensor q, torch::Tensor kv, torch::Tensor k_rope, double scale,
+        bool causal, c10::optional<torch::Tensor> lengths,
+        c10::optional<torch::Tensor> past);
 
 namespace {
 
@@ -107,6 +111,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           py::arg("interleaved") = false, py::arg("offset") = 0,
           py::arg("inverse") = false, py::arg("scale") = 1.0,
           py::arg("in_place") = false);
+    m.def("latent_attention", &latent_attention_op, py::arg("q"),
+          py::arg("kv"), py::arg("k_rope"), py::arg("scale"),
+          py::arg("causal") = false, py::arg("lengths") = py::none(),
+          py::arg("past") = py::none());
     m.def("_debug_mfma_tile", &debug_mfma_tile);
     m.def("_debug_mfma32_raw", &debug_mfma32_raw);
     m.def("_debug_tr16_raw", &debug_tr16_raw);

@@ -181,3 +181,83 @@ def rotary(q: Tensor, positions: Tensor, freqs: Tensor,
         return out
 
     return _turn(q), None if k is None else _turn(k)
+
+
+def _softmax_seen(scores: Tensor, seen: Tensor) -> Tensor:
+    """Softmax over the seen scores; a row that sees nothing gets zeros."""
+    scores = scores.masked_fill(~seen, float("-inf"))
+    top = scores.amax(-1, keepdim=True)
+    weight = torch.exp(scores - top.masked_fill(top == float("-inf"), 0.0))
+    total = weight.sum(-1, keepdim=True)
+    return weight / total.masked_fill(total == 0.0, 1.0)
+
+
+def check_latent_attention(q: Tensor, kv: Tensor, k_rope: Tensor,
+                           scale: float, lengths: Optional[Tensor],
+                           past: Optional[Tensor]):
+    """The argument checks of the latent attention kernel (CPU path)."""
+    op = "latent_attention"
+    if not (q.dtype == kv.dtype == k_rope.dtype):
+        raise TypeError(f"{op}: q, kv and k_rope must have one type")
+    if any(t is not None and t.device != q.device
+           for t in (kv, k_rope, lengths, past)):
+        raise ValueError(f"{op}: tensors on different devices")
+    _check_inference(op, q, kv, k_rope)
+    if q.dim() != 4 or kv.dim() != 4 or k_rope.dim() != 3:
+        raise ValueError(f"{op}: q and kv must be [B, S, H, D], "
+                         "k_rope [B, S, D]")
+    b, sq, h, _ = q.shape
+    sk, nope = kv.shape[1], q.shape[3] - k_rope.shape[2]
+    if nope not in (64, 128) or k_rope.shape[2] not in (32, 64) \
+            or kv.shape[3] != 2 * nope:
+        raise ValueError(
+            f"{op}: head parts must be 64 or 128 plain and 32 or 64 rotary "
+            "columns with as many values as plain ones, got q "
+            f"{q.shape[3]}, kv {kv.shape[3]}, k_rope {k_rope.shape[2]}")
+    if kv.shape[:3] != (b, sk, h) or k_rope.shape[:2] != (b, sk):
+        raise ValueError(f"{op}: q {list(q.shape)}, kv {list(kv.shape)} and "
+                         f"k_rope {list(k_rope.shape)} do not match")
+    if not 0.0 < scale < math.inf:
+        raise ValueError(f"{op}: scale must be positive")
+    for t in (lengths, past):
+        if t is None:
+            continue
+        if t.dtype != torch.int32:
+            raise TypeError(f"{op}: lengths and past must be int32")
+        if t.shape != (b,):
+            raise ValueError(f"{op}: lengths and past must be one a sequence")
+    if lengths is not None and past is None and sq != sk:
+        raise ValueError(f"{op}: lengths with fewer or more queries than "
+                         "keys need past")
+
+
+def latent_attention(q: Tensor, kv: Tensor, k_rope: Tensor, scale: float,
+                     causal: bool = False, lengths: Optional[Tensor] = None,
+                     past: Optional[Tensor] = None) -> Tensor:
+    """Attention with keys ``[kv[.., :DN] | k_rope]`` and values
+    ``kv[.., DN:]``; the rotary key part is shared by all heads."""
+    check_latent_attention(q, kv, k_rope, scale, lengths, past)
+    b, sq, h, _ = q.shape
+    sk, nope = kv.shape[1], q.shape[3] - k_rope.shape[2]
+    if sk == 0:
+        return q.new_zeros(b, sq, h, nope)
+    length = torch.full((b, 1), sk, dtype=torch.int64, device=q.device) \
+        if lengths is None else lengths.long().clamp(0, sk).reshape(b, 1)
+    first = torch.full_like(length, sk - sq) if past is None \
+        else past.long().reshape(b, 1)
+    at = first + torch.arange(sq, device=q.device)
+    key = torch.arange(sk, device=q.device)
+    seen = ((at >= 0) & (at < length)).unsqueeze(-1) \
+        & (key < length).unsqueeze(1)
+    if causal:
+        seen = seen & (key <= at.unsqueeze(-1))
+    # what lies behind a sequence never reaches its sums
+    inside = (key < length).reshape(b, 1, sk, 1)
+    heads = kv.float().transpose(1, 2).masked_fill(~inside, 0.0)
+    rope = k_rope.float().unsqueeze(1).masked_fill(~inside, 0.0)
+    full = torch.cat((heads[..., :nope], rope.expand(-1, h, -1, -1)), dim=-1)
+    scores = torch.matmul(q.float().transpose(1, 2),
+                          full.transpose(-1, -2)) * scale
+    weight = _softmax_seen(scores, seen.unsqueeze(1))
+    out = torch.matmul(weight, heads[..., nope:].contiguous())
+    return out.transpose(1, 2).contiguous().to(q.dtype)
