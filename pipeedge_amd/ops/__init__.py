@@ -274,3 +274,27 @@ def latent_attention(q: Tensor, kv: Tensor, k_rope: Tensor, *,
         scale = 1.0 / math.sqrt(max(q.shape[-1], 1))
     run = _hip.latent_attention if _use_hip(q) else torch_ref.latent_attention
     return run(q, kv, k_rope, scale, causal, lengths, past)
+
+
+def latent_cache_attention(q: Tensor, cache: Tensor, block_table: Tensor,
+                           lengths: Tensor, *, latent_dim: int,
+                           scale: float) -> Tensor:
+    """Attention over latent vectors in absorbed form, for single tokens.
+
+    ``cache`` [pages, page size, R + DR] holds a latent vector and the rotated
+    shared key columns of each token (R = ``latent_dim`` 256 or 512, DR 32 or
+    64, bfloat16 or float16, rows contiguous and at multiples of 16 bytes, any
+    page size), ``block_table`` (int32 [B, P]) the pages of each sequence and
+    ``lengths`` (int32 [B]) its tokens, the ``Sq`` newest of which are the
+    queries. ``q`` [B, Sq, H, R + DR] are their heads with the key projection
+    absorbed, [q_nope W_uk | q_rope]; ``scale`` is that of the expanded form.
+    Returns [B, Sq, H, R], the weighted latent vectors, to which the value
+    projection is applied afterwards. Query i sees tokens up to its own
+    position, lengths - Sq + i; one before the start comes back zero, as does
+    an empty sequence. Table entries behind a sequence are not read. A length
+    that the table cannot hold, or a page number that the cache does not have,
+    makes that sequence's outputs NaN. Up to 128 (query, head) pairs share one
+    pass over the cache; a few tokens at a time are what it is made for."""
+    run = _hip.latent_cache_attention if _use_hip(q) \
+        else torch_ref.latent_cache_attention
+    return run(q, cache, block_table, lengths, latent_dim, scale)

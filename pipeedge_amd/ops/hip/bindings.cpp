@@ -41,6 +41,9 @@ torch::Tensor latent_attention_op(
         torch::Tensor q, torch::Tensor kv, torch::Tensor k_rope, double scale,
         bool causal, c10::optional<torch::Tensor> lengths,
         c10::optional<torch::Tensor> past);
+torch::Tensor latent_cache_attention_op(
+        torch::Tensor q, torch::Tensor cache, torch::Tensor block_table,
+        torch::Tensor lengths, int64_t latent_dim, double scale);
 
 namespace {
 
@@ -115,6 +118,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           py::arg("kv"), py::arg("k_rope"), py::arg("scale"),
           py::arg("causal") = false, py::arg("lengths") = py::none(),
           py::arg("past") = py::none());
+    m.def("latent_cache_attention", &latent_cache_attention_op, py::arg("q"),
+          py::arg("cache"), py::arg("block_table"), py::arg("lengths"),
+          py::arg("latent_dim"), py::arg("scale"));
     m.def("_debug_mfma_tile", &debug_mfma_tile);
     m.def("_debug_mfma32_raw", &debug_mfma32_raw);
     m.def("_debug_tr16_raw", &debug_tr16_raw);

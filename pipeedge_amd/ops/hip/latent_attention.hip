@@ -7,8 +7,8 @@
 // the keys in tiles of 64. Both products are computed transposed (tokens or
 // value columns as the rows, queries as the columns of 32x32x16 MFMAs), so a
 // lane holds scores of one query only: softmax needs one exchange between
-// the halves of a wave, and the weights become the second product's operand
-// in registers. Tiles go to LDS by LDS-DMA while the previous one is used;
+// the halves of a wave, and the weights are the second product's operand as
+// they are, without leaving their lane. Tiles go to LDS by LDS-DMA while the previous one is used;
 // the shared rotary key is staged as it is and never copied per head.
 // Bound by the matrix cores and the LDS reads that feed them.
 #include <torch/extension.h>
@@ -44,7 +44,7 @@ __global__ __launch_bounds__(256, 2) void latent_attention_kernel(
     typedef LatentSoftmax<T> softmax;
     // two buffers of [nope | rope | value] images
     constexpr int TILE = KEYS * (2 * DN + DR);
-    __shared__ T smem[2 * TILE];
+    __shared__ __attribute__((aligned(256))) T smem[2 * TILE];
 
     const int id = xcd_contiguous(blockIdx.x, gridDim.x);
     const int bh = id / a.row_blocks;
@@ -113,11 +113,15 @@ __global__ __launch_bounds__(256, 2) void latent_attention_kernel(
     f32x16 acc[NT] = {};
     float top = -INFINITY, sub = 0.0f, total = 0.0f;
 
+    const unsigned lds = latent_lds(smem);
     if (tiles > 0) stage(0, 0);
     for (int t = 0; t < tiles; ++t) {
-        const T* nope = smem + (t & 1) * TILE;
-        const T* rope = nope + KEYS * DN;
-        const T* value = rope + KEYS * DR;
+        const unsigned image = lds + (t & 1) * TILE * 2;
+        const unsigned nope = latent_row_base<CN, 32>(image, lane);
+        const unsigned rope =
+            latent_row_base<CR, 32>(image + KEYS * DN * 2, lane);
+        const unsigned value = latent_column_base<CN, 32>(
+            image + KEYS * (DN + DR) * 2, lane);
         // this wave's part of tile t has arrived; behind the barrier all
         // parts have, and every wave is done with the other buffer
         latent_arrive();
@@ -130,14 +134,14 @@ __global__ __launch_bounds__(256, 2) void latent_attention_kernel(
         for (int i = 0; i < DN / 16; ++i)
             #pragma unroll
             for (int m = 0; m < 2; ++m)
-                s[m] = latent_mfma(latent_row_read<T, CN>(
-                    nope, m * 32 + l31, 2 * i + hi), bq[i], s[m]);
+                s[m] = latent_mfma(latent_row_read<T, CN, 32>(nope, m * 32, i),
+                                   bq[i], s[m]);
         #pragma unroll
         for (int i = 0; i < DR / 16; ++i)
             #pragma unroll
             for (int m = 0; m < 2; ++m)
-                s[m] = latent_mfma(latent_row_read<T, CR>(
-                    rope, m * 32 + l31, 2 * i + hi), bq[DN / 16 + i], s[m]);
+                s[m] = latent_mfma(latent_row_read<T, CR, 32>(rope, m * 32, i),
+                                   bq[DN / 16 + i], s[m]);
 
         if (__any(limit < tok0 + KEYS - 1)) {
             #pragma unroll
@@ -178,11 +182,14 @@ __global__ __launch_bounds__(256, 2) void latent_attention_kernel(
         for (int m = 0; m < 2; ++m)
             #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                const v8 w = latent_weights<T>(s[m], c);
+                float p[8];
+                #pragma unroll
+                for (int j = 0; j < 8; ++j) p[j] = s[m][8 * c + j];
+                const v8 w = latent_weights<T>(p);
                 #pragma unroll
                 for (int n = 0; n < NT; ++n)
-                    acc[n] = latent_mfma(latent_column_read<T, CN>(
-                        value, m * 32 + c * 16, n * 32, lane), w, acc[n]);
+                    acc[n] = latent_mfma(latent_column_read<T, CN, 32>(
+                        value, m * 32 + c * 16, n), w, acc[n]);
             }
     }
 

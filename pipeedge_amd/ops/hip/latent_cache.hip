@@ -1,0 +1,629 @@
+// Latent attention, absorbed form: the projections to keys and values are
+// moved to the query and output side, so every head attends to the cached
+// vectors themselves, whose first R columns are also the values:
+//   out[i, h] = softmax_t(scale * q[i, h] . cache[t]) cache[t][:R]
+// The rows of a product are (query, head) pairs, all of one sequence, so one
+// pass over the cache serves all heads; 16 heads are bound by memory, 128 by
+// the matrix cores.
+//
+// Work is cut into tiles of 64 cached tokens, numbered through all sequences
+// and row groups, and each of a fixed number of blocks takes an equal run of
+// them, across sequences where it falls so: lengths stay on the device, and
+// ragged batches are balanced to within a tile. A run inside one (sequence,
+// row group) is a segment; a segment that covers all its tiles is written to
+// the output, others leave partial sums in fp32 that a second kernel joins
+// in a fixed order.
+//
+// Both products are transposed as in the expanded form, on 16x16x32 MFMAs: a
+// wave owns 16 rows, a lane holds one row's scores, and the weights are the
+// second operand as they are. One LDS image of a tile serves both products,
+// read by rows for the scores and by columns, through the transposing reads,
+// for the values. The accumulators take R / 4 registers and the query
+// operands (R + DR) / 8, so two waves share a SIMD: 8 waves of one block, 128
+// rows, use a tile of 64 tokens together. With fewer rows the waves also
+// split a tile's tokens, 32 each, and join their sums at the segment's end;
+// up to 16 rows a wave loads its own tokens, two tiles ahead, and waits for
+// nobody else.
+#include <torch/extension.h>
+
+#include <c10/core/DeviceGuard.h>
+
+#include "latent_common.h"
+
+namespace {
+
+constexpr int KEYS = 64;            // tokens a tile
+
+struct CacheArgs {
+    const void* q;                  // [B, Sq, H, R + DR]
+    const void* cache;              // [pages, page size, R + DR]
+    const int* table;               // [B, table_width]
+    const int* lengths;             // [B]
+    void* out;                      // [B, Sq, H, R]
+    float* part;                    // [segments][rows][R] partial sums
+    float2* part_stat;              // [segments][rows] reference, total
+    long q_b, q_s, q_h, c_p, c_t, t_b;      // strides in elements
+    long pages;
+    int page_size, page_shift;      // shift -1: not a power of two
+    bool page_of_groups;            // a multiple of 8 tokens
+    int B, H, Sq, table_width;
+    int rows;                       // Sq * H
+    int row_groups;                 // ceil(rows / rows a block)
+    float scale;                    // times log2(e)
+};
+
+// Tiles of a sequence. A length that the table cannot hold counts as what it
+// can hold; its outputs are NaN.
+__device__ __forceinline__ int cache_length(const CacheArgs& a, int b) {
+    const long most = (long)a.table_width * a.page_size;
+    return (int)min((long)max(a.lengths[b], 0), most);
+}
+__device__ __forceinline__ int cache_tiles(const CacheArgs& a, int b) {
+    return b < a.B ? (cache_length(a, b) + KEYS - 1) / KEYS : 0;
+}
+
+__device__ __forceinline__ int wave_scan(int v, int lane) {
+    #pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const int up = __shfl_up(v, d);
+        if (lane >= d) v += up;
+    }
+    return v;
+}
+
+__device__ __forceinline__ long cache_total(const CacheArgs& a, int lane) {
+    long total = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 64)
+        total += __builtin_amdgcn_readlane(
+            wave_scan(cache_tiles(a, b0 + lane), lane), 63);
+    return total * a.row_groups;
+}
+
+// Place of tile number `at` (of all row groups and sequences): the sequence
+// and the number of its first tile.
+__device__ __forceinline__ void cache_find(const CacheArgs& a, long at,
+                                           int lane, int& seq, long& first) {
+    long before = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 64) {
+        const int mine = cache_tiles(a, b0 + lane);
+        const int upto = wave_scan(mine, lane);
+        const long end = before + (long)upto * a.row_groups;
+        const unsigned long long past = __ballot(end > at);
+        if (past) {
+            const int l = __builtin_ctzll(past);
+            seq = b0 + l;
+            first = before + (long)(__builtin_amdgcn_readlane(upto, l)
+                     - __builtin_amdgcn_readlane(mine, l)) * a.row_groups;
+            return;
+        }
+        before += (long)__builtin_amdgcn_readlane(upto, 63) * a.row_groups;
+    }
+    seq = a.B;
+    first = before;
+}
+
+// tiles of block g: run_start(g) .. run_start(g + 1)
+__device__ __forceinline__ long run_start(long total, int g, int blocks) {
+    return total / blocks * g + min((long)g, total % blocks);
+}
+// the block that has tile `at`
+__device__ __forceinline__ int run_block(long total, long at, int blocks) {
+    const long each = total / blocks, extra = total % blocks;
+    if (at < extra * (each + 1)) return (int)(at / (each + 1));
+    return (int)(extra + (at - extra * (each + 1)) / each);
+}
+
+// Where the 8 tokens of one group lie: the address of the first, and the
+// number of the last that holds one (tokens behind the last of the sequence
+// are read as the last one, so that no padding reaches a product).
+struct CacheGroup {
+    const char* at;
+    int last;
+};
+
+// WR groups of 16 rows times WT waves a group, KEYS / WT tokens each.
+template <typename T, int R, int DR, int WR, int WT>
+__global__ __launch_bounds__(64 * WR * WT, 2)
+void latent_cache_kernel(CacheArgs a) {
+    constexpr int CL = R / 8, CR = DR / 8;      // chunks of a row's parts
+    constexpr int NT = R / 16;                  // output tiles
+    constexpr int TOKENS = KEYS / WT;           // tokens a wave and tile
+    constexpr int SUB = TOKENS / 16;            // score columns
+    constexpr int GROUPS = TOKENS / 8 / WR;     // 8 tokens each, to load
+    constexpr int TILE = TOKENS * (R + DR);
+    // the waves of one row group load and use their tokens alone
+    constexpr bool ALONE = WR == 1;
+    constexpr int PIECES = GROUPS * CL / 8 + GROUPS * CR / 8;
+    static_assert(!ALONE || (GROUPS == 4 && PIECES < 64), "counted waits");
+    typedef typename LatentVec<T>::v8 v8;
+    typedef LatentSoftmax<T> softmax;
+    // WT shares of two buffers of [latent | rope] images
+    __shared__ __attribute__((aligned(256))) T smem[WT * 2 * TILE];
+
+    const int tid = threadIdx.x;
+    const int lane = tid & 63, l15 = lane & 15, quad = lane >> 4;
+    const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int group = wid % WR, share = wid / WR;
+    T* const images = smem + share * 2 * TILE;
+    const unsigned lds = latent_lds(images);
+
+    const long total = cache_total(a, lane);
+    long at = run_start(total, blockIdx.x, gridDim.x);
+    const long end = run_start(total, blockIdx.x + 1, gridDim.x);
+    if (at >= end) return;
+    int seq;
+    long first;
+    cache_find(a, at, lane, seq, first);
+
+    while (at < end) {
+        const int len = cache_length(a, seq);
+        const int tiles = (len + KEYS - 1) / KEYS;
+        if (tiles == 0) { ++seq; continue; }
+        const int rg = (int)((at - first) / tiles);
+        const long base = first + (long)rg * tiles;
+        const int t0 = (int)(at - base);
+        const int t1 = (int)min((long)tiles, end - base);
+
+        // this lane's row and the last token that it sees
+        const int row = (rg * WR + group) * 16 + l15;
+        const bool live = (rg * WR + group) * 16 < a.rows;
+        const int rowc = min(row, a.rows - 1);
+        const int qi = rowc / a.H, h = rowc - qi * a.H;
+        const int limit = len - a.Sq + qi;
+        v8 bq[(R + DR) / 32];
+        {
+            const T* p = reinterpret_cast<const T*>(a.q) + seq * a.q_b
+                         + qi * a.q_s + h * a.q_h + quad * 8;
+            #pragma unroll
+            for (int i = 0; i < (R + DR) / 32; ++i)
+                bq[i] = *reinterpret_cast<const v8*>(p + i * 32);
+        }
+
+        // A page number that the cache does not have reads page 0 and
+        // spoils the output, as does a length that the table cannot hold.
+        bool bad = a.lengths[seq] > len;
+        const int* table = a.table + seq * a.t_b;
+        const auto page_at = [&](int slot) {
+            int page = table[slot];
+            if (page < 0 || page >= a.pages) { bad = true; page = 0; }
+            return reinterpret_cast<const char*>(a.cache) + page * a.c_p * 2;
+        };
+        const int step = (int)a.c_t * 2;        // bytes from token to token
+        const auto stage = [&](int t, int buf) {
+            T* image = images + buf * TILE + group * GROUPS * 8 * R;
+            T* rotary = images + buf * TILE + TOKENS * R
+                        + group * GROUPS * 8 * DR;
+            const int tok0 = t * KEYS + share * TOKENS + group * GROUPS * 8;
+            // piece p of the latent part has rows p * PR .. of this wave's
+            // tokens, of the rotary part rows p * RR ..
+            constexpr int PR = 64 / CL, RR = 64 / CR;
+            const auto latent_chunk = [&](int r) {
+                return ((lane % CL) ^ latent_key<CL>(group * GROUPS * 8 + r))
+                       * 16;
+            };
+            const auto rotary_chunk = [&](int r) {
+                return R * 2 + ((lane % CR)
+                    ^ latent_key<CR>(group * GROUPS * 8 + r)) * 16;
+            };
+            if (a.page_of_groups) {
+                // groups of 8 tokens never straddle a page: their places
+                // are the same for all lanes and live in scalar registers
+                CacheGroup from[GROUPS];
+                #pragma unroll
+                for (int g = 0; g < GROUPS; ++g) {
+                    // behind the end, the last group once more
+                    const int tok = min(tok0 + g * 8, (len - 1) & ~7);
+                    const int slot = a.page_shift >= 0 ? tok >> a.page_shift
+                                                       : tok / a.page_size;
+                    from[g].at = page_at(slot)
+                        + (long)(tok - slot * a.page_size) * a.c_t * 2;
+                    from[g].last = len - 1 - tok;
+                }
+                #pragma unroll
+                for (int p = 0; p < GROUPS * 8 / PR; ++p) {
+                    const int r = p * PR + (PR == 1 ? 0 : lane / CL);
+                    const CacheGroup& f = from[p * PR / 8];
+                    latent_lds_load(
+                        f.at + min(r % 8, f.last) * step + latent_chunk(r),
+                        image + p * PR * R);
+                }
+                #pragma unroll
+                for (int p = 0; p < (GROUPS * 8 + RR - 1) / RR; ++p) {
+                    const int r = p * RR + lane / CR;
+                    CacheGroup f = from[p * RR / 8];
+                    if (RR == 16 && GROUPS > 1 && lane >= 32)
+                        f = from[(p * RR / 8 + 1) % GROUPS];
+                    if (r < GROUPS * 8)
+                        latent_lds_load(
+                            f.at + min(r % 8, f.last) * step
+                            + rotary_chunk(r), rotary + p * RR * DR);
+                }
+            } else {
+                // any other page size: lane l finds token l
+                const int tok = min(tok0 + lane % (GROUPS * 8), len - 1);
+                const int slot = tok / a.page_size;
+                const long place = page_at(slot)
+                    - reinterpret_cast<const char*>(a.cache)
+                    + (long)(tok - slot * a.page_size) * a.c_t * 2;
+                #pragma unroll
+                for (int p = 0; p < GROUPS * 8 / PR; ++p) {
+                    const int r = p * PR + lane / CL;
+                    latent_lds_load(
+                        reinterpret_cast<const char*>(a.cache)
+                        + __shfl(place, r) + latent_chunk(r),
+                        image + p * PR * R);
+                }
+                #pragma unroll
+                for (int p = 0; p < (GROUPS * 8 + RR - 1) / RR; ++p) {
+                    const int r = p * RR + lane / CR;
+                    const long from = __shfl(place, r);
+                    if (r < GROUPS * 8)
+                        latent_lds_load(
+                            reinterpret_cast<const char*>(a.cache) + from
+                            + rotary_chunk(r), rotary + p * RR * DR);
+                }
+            }
+        };
+
+        f32x4 acc[NT] = {};
+        float top = -INFINITY, sub = 0.0f, sum = 0.0f;
+        // every wave is done with the LDS of the segment before
+        __syncthreads();
+        stage(t0, t0 & 1);
+        if (ALONE && t0 + 1 < t1) stage(t0 + 1, (t0 + 1) & 1);
+        for (int t = t0; t < t1; ++t) {
+            if constexpr (ALONE) {
+                // all but the next tile's pieces have arrived
+                if (t + 1 < t1)
+                    asm volatile("s_waitcnt vmcnt(%0)" ::"i"(PIECES)
+                                 : "memory");
+                else
+                    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            } else {
+                latent_arrive();
+                if (t + 1 < t1) stage(t + 1, (t + 1) & 1);
+            }
+            const unsigned image = lds + (t & 1) * TILE * 2;
+            const unsigned latent = latent_row_base<CL, 16>(image, lane);
+            const unsigned rope = latent_row_base<CR, 16>(
+                image + TOKENS * R * 2, lane);
+            const unsigned value = latent_column_base<CL, 16>(image, lane);
+            const int tok0 = t * KEYS + share * TOKENS;
+
+            if (live) {
+            f32x4 s[SUB] = {};
+            #pragma unroll
+            for (int i = 0; i < R / 32; ++i)
+                #pragma unroll
+                for (int m = 0; m < SUB; ++m)
+                    s[m] = latent_mfma(latent_row_read<T, CL, 16>(
+                        latent, m * 16, i), bq[i], s[m]);
+            #pragma unroll
+            for (int i = 0; i < DR / 32; ++i)
+                #pragma unroll
+                for (int m = 0; m < SUB; ++m)
+                    s[m] = latent_mfma(latent_row_read<T, CR, 16>(
+                        rope, m * 16, i), bq[R / 32 + i], s[m]);
+
+            if (__any(limit < tok0 + TOKENS - 1)) {
+                #pragma unroll
+                for (int m = 0; m < SUB; ++m)
+                    #pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (tok0 + m * 16 + quad * 4 + i > limit)
+                            s[m][i] = -INFINITY;
+            }
+            float peak = -INFINITY;
+            #pragma unroll
+            for (int m = 0; m < SUB; ++m)
+                #pragma unroll
+                for (int i = 0; i < 4; ++i) peak = fmaxf(peak, s[m][i]);
+            peak = fmaxf(peak, __shfl_xor(peak, 16));
+            peak = fmaxf(peak, __shfl_xor(peak, 32)) * a.scale;
+            if (__any(peak > top + softmax::SLACK)) {
+                const float next = fmaxf(top, peak);
+                const float turn = top == -INFINITY
+                    ? 0.0f : __builtin_amdgcn_exp2f(top - next);
+                top = next;
+                sub = next == -INFINITY ? 0.0f : next - softmax::BIAS;
+                sum *= turn;
+                #pragma unroll
+                for (int n = 0; n < NT; ++n)
+                    #pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[n][i] *= turn;
+            }
+            #pragma unroll
+            for (int m = 0; m < SUB; ++m)
+                #pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    s[m][i] = __builtin_amdgcn_exp2f(
+                        fmaf(s[m][i], a.scale, -sub));
+                    sum += s[m][i];
+                }
+            #pragma unroll
+            for (int m = 0; m < SUB; m += 2) {
+                float p[8];
+                #pragma unroll
+                for (int j = 0; j < 8; ++j) p[j] = s[m + j / 4][j % 4];
+                const v8 w = latent_weights<T>(p);
+                #pragma unroll
+                for (int n = 0; n < NT; ++n)
+                    acc[n] = latent_mfma(latent_column_read<T, CL, 16>(
+                        value, m * 16, n), w, acc[n]);
+            }
+            }
+            if (ALONE && t + 2 < t1) stage(t + 2, t & 1);
+        }
+        sum += __shfl_xor(sum, 16);
+        sum += __shfl_xor(sum, 32);
+        // whichever wave loaded from the bad page
+        if (__syncthreads_or(bad)) sum = NAN;
+
+        if constexpr (WT == 2) {
+            // the second wave of a group hands its sums to the first; the
+            // barrier above ended all use of the tiles
+            constexpr int STEP = 64 * WR;
+            float* give = reinterpret_cast<float*>(smem) + group * 64 + lane;
+            float* stat = give + STEP * NT * 4;
+            static_assert((NT * 4 + 2) * STEP * 4 <= WT * 2 * TILE * 2,
+                          "the sums must fit in the tiles' LDS");
+            if (share == 1) {
+                #pragma unroll
+                for (int n = 0; n < NT; ++n)
+                    #pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        give[(n * 4 + i) * STEP] = acc[n][i];
+                stat[0] = top;
+                stat[STEP] = sum;
+            }
+            __syncthreads();
+            if (share == 0) {
+                const float top2 = stat[0], sum2 = stat[STEP];
+                const float next = fmaxf(top, top2);
+                // a share that saw no token has nothing to give
+                const float f1 = top == -INFINITY
+                    ? 0.0f : __builtin_amdgcn_exp2f(top - next);
+                const float f2 = top2 == -INFINITY
+                    ? 0.0f : __builtin_amdgcn_exp2f(top2 - next);
+                top = next;
+                sum = (sum == sum ? sum * f1 : sum)
+                      + (sum2 == sum2 ? sum2 * f2 : sum2);
+                #pragma unroll
+                for (int n = 0; n < NT; ++n)
+                    #pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        acc[n][i] = acc[n][i] * f1
+                                    + give[(n * 4 + i) * STEP] * f2;
+            }
+        }
+
+        const bool whole = t0 == 0 && t1 == tiles;
+        if (share == 0 && row < a.rows) {
+            if (whole) {
+                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                T* out = reinterpret_cast<T*>(a.out)
+                         + ((long)seq * a.rows + row) * R + quad * 4;
+                #pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    typename LatentVec<T>::v4 o;
+                    #pragma unroll
+                    for (int j = 0; j < 4; ++j) o[j] = (T)(acc[n][j] * inv);
+                    *reinterpret_cast<typename LatentVec<T>::v4*>(
+                        out + n * 16) = o;
+                }
+            } else {
+                // block and work item numbers only grow together, so their
+                // sum is a slot that no other segment has
+                const long slot = (long)blockIdx.x
+                    + (long)seq * a.row_groups + rg;
+                const long at_row = slot * (16 * WR) + group * 16 + l15;
+                float* out = a.part + at_row * R + quad * 4;
+                #pragma unroll
+                for (int n = 0; n < NT; ++n)
+                    *reinterpret_cast<f32x4*>(out + n * 16) = acc[n];
+                if (quad == 0) a.part_stat[at_row] = make_float2(top, sum);
+            }
+        }
+        at = base + t1;
+        if (t1 == tiles && rg + 1 == a.row_groups) {
+            first += (long)tiles * a.row_groups;
+            ++seq;
+        }
+    }
+}
+
+// Joins the segments of one row a wave: out = sum 2^(top_i - top) part_i /
+// sum 2^(top_i - top) sum_i, over the blocks in their order. Sequences that
+// hold nothing get zeros; whole segments are there already.
+template <typename T, int R>
+__global__ __launch_bounds__(256) void latent_cache_join_kernel(
+        CacheArgs a, int block_rows, int blocks) {
+    constexpr int E = R / 64;                   // elements a lane
+    typedef float vec __attribute__((ext_vector_type(E)));
+    typedef T ovec __attribute__((ext_vector_type(E)));
+    const int lane = threadIdx.x & 63;
+    const int seq = blockIdx.y;
+    const int row = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= a.rows) return;
+    T* out = reinterpret_cast<T*>(a.out) + ((long)seq * a.rows + row) * R
+             + lane * E;
+    const int tiles = cache_tiles(a, seq);
+    if (tiles == 0) {
+        *reinterpret_cast<ovec*>(out) = ovec{};
+        return;
+    }
+    const int rg = row / block_rows;
+    long total = 0, first = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 64) {
+        const int mine = cache_tiles(a, b0 + lane);
+        const int upto = wave_scan(mine, lane);
+        if (seq >= b0 && seq < b0 + 64)
+            first = total + __builtin_amdgcn_readlane(upto, seq - b0) - tiles;
+        total += __builtin_amdgcn_readlane(upto, 63);
+    }
+    total *= a.row_groups;
+    first = first * a.row_groups + (long)rg * tiles;
+    const int g0 = run_block(total, first, blocks);
+    const int g1 = run_block(total, first + tiles - 1, blocks);
+    if (g0 == g1) return;
+    const long slot0 = (long)seq * a.row_groups + rg;
+    const int r = row - rg * block_rows;
+    float top = -INFINITY;
+    for (int g = g0; g <= g1; ++g)
+        top = fmaxf(top, a.part_stat[(slot0 + g) * block_rows + r].x);
+    float sum = 0.0f;
+    vec acc = {};
+    for (int g = g0; g <= g1; ++g) {
+        const long at = (slot0 + g) * block_rows + r;
+        const float2 st = a.part_stat[at];
+        const float f = st.x == -INFINITY
+            ? 0.0f : __builtin_amdgcn_exp2f(st.x - top);
+        sum += st.y == st.y ? st.y * f : st.y;
+        acc += *reinterpret_cast<const vec*>(a.part + at * R + lane * E) * f;
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    ovec o;
+    #pragma unroll
+    for (int j = 0; j < E; ++j) o[j] = (T)(acc[j] * inv);
+    *reinterpret_cast<ovec*>(out) = o;
+}
+
+bool cache_rows_ok(const torch::Tensor& x) {
+    bool ok = reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0 &&
+              x.stride(-1) == 1;
+    for (int64_t d = 0; d + 1 < x.dim(); ++d)
+        ok = ok && (x.size(d) == 1 || x.stride(d) % 8 == 0);
+    return ok;
+}
+
+template <typename T, int R, int DR, int WR, int WT>
+void cache_launch_shape(const CacheArgs& a, int blocks) {
+    hipLaunchKernelGGL((latent_cache_kernel<T, R, DR, WR, WT>), dim3(blocks),
+                       dim3(64 * WR * WT), 0, pe_current_stream(), a);
+    hipLaunchKernelGGL((latent_cache_join_kernel<T, R>),
+                       dim3((a.rows + 3) / 4, a.B), dim3(256), 0,
+                       pe_current_stream(), a, 16 * WR, blocks);
+}
+
+template <typename T, int R, int DR>
+void cache_launch(const CacheArgs& a, int block_rows, int blocks) {
+    if (block_rows == 128) cache_launch_shape<T, R, DR, 8, 1>(a, blocks);
+    else if (block_rows == 64) cache_launch_shape<T, R, DR, 4, 2>(a, blocks);
+    else if (block_rows == 32) cache_launch_shape<T, R, DR, 2, 2>(a, blocks);
+    else cache_launch_shape<T, R, DR, 1, 2>(a, blocks);
+}
+
+template <typename T>
+void cache_dispatch(const CacheArgs& a, int latent, int rope, int block_rows,
+                    int blocks) {
+    if (latent == 512 && rope == 64)
+        cache_launch<T, 512, 64>(a, block_rows, blocks);
+    else if (latent == 512)
+        cache_launch<T, 512, 32>(a, block_rows, blocks);
+    else if (rope == 64)
+        cache_launch<T, 256, 64>(a, block_rows, blocks);
+    else
+        cache_launch<T, 256, 32>(a, block_rows, blocks);
+}
+
+}  // namespace
+
+torch::Tensor latent_cache_attention_op(
+        torch::Tensor q, torch::Tensor cache, torch::Tensor block_table,
+        torch::Tensor lengths, int64_t latent_dim, double scale) {
+    TORCH_CHECK_VALUE(q.is_cuda(),
+                      "latent_cache_attention: GPU tensors required");
+    const c10::DeviceGuard guard(q.device());
+    const auto dtype = q.scalar_type();
+    TORCH_CHECK_TYPE((dtype == torch::kBFloat16 || dtype == torch::kHalf) &&
+                     cache.scalar_type() == dtype,
+                     "latent_cache_attention: q and cache must be both "
+                     "bfloat16 or both float16");
+    TORCH_CHECK_TYPE(block_table.scalar_type() == torch::kInt &&
+                     lengths.scalar_type() == torch::kInt,
+                     "latent_cache_attention: block_table and lengths must "
+                     "be int32");
+    TORCH_CHECK_VALUE(cache.device() == q.device() &&
+                      block_table.device() == q.device() &&
+                      lengths.device() == q.device(),
+                      "latent_cache_attention: tensors on different devices");
+    TORCH_CHECK_VALUE(!(at::GradMode::is_enabled() &&
+                        (q.requires_grad() || cache.requires_grad())),
+                      "latent_cache_attention: inference only, an input "
+                      "requires a gradient");
+    TORCH_CHECK_VALUE(q.dim() == 4 && cache.dim() == 3 &&
+                      q.size(3) == cache.size(2),
+                      "latent_cache_attention: q must be [B, Sq, H, D] and "
+                      "cache [pages, page size, D], got ", q.sizes(), " and ",
+                      cache.sizes());
+    const int64_t B = q.size(0), Sq = q.size(1), H = q.size(2);
+    const int64_t rope = q.size(3) - latent_dim;
+    TORCH_CHECK_VALUE((latent_dim == 256 || latent_dim == 512) &&
+                      (rope == 32 || rope == 64),
+                      "latent_cache_attention: rows must be 256 or 512 "
+                      "latent and 32 or 64 rotary columns, got ", latent_dim,
+                      " and ", rope);
+    TORCH_CHECK_VALUE(block_table.dim() == 2 && block_table.size(0) == B &&
+                      lengths.dim() == 1 && lengths.size(0) == B,
+                      "latent_cache_attention: block_table must be [B, P] "
+                      "and lengths [B]");
+    TORCH_CHECK_VALUE(scale > 0.0 && std::isfinite(scale),
+                      "latent_cache_attention: scale must be positive");
+    auto out = torch::empty({B, Sq, H, latent_dim}, q.options());
+    if (out.numel() == 0) return out;
+    const int64_t page = cache.size(1), width = block_table.size(1);
+    if (page == 0 || width == 0) {
+        // nothing can be held: every length other than zero is too long
+        return out.copy_(torch::where(
+            lengths > 0, NAN, 0.0).reshape({B, 1, 1, 1}));
+    }
+    TORCH_CHECK_VALUE(cache.size(0) > 0,
+                      "latent_cache_attention: the cache has no page");
+    TORCH_CHECK_VALUE(cache_rows_ok(cache),
+                      "latent_cache_attention: cache rows must be contiguous "
+                      "and lie at multiples of 16 bytes");
+    TORCH_CHECK_VALUE(page * width < (1L << 31) - 128 && B < 65536 &&
+                      Sq * H < (1L << 24) && cache.stride(1) < (1L << 26),
+                      "latent_cache_attention: too many tokens or rows");
+    const auto qa = cache_rows_ok(q) ? q
+        : q.clone(at::MemoryFormat::Contiguous);
+    const auto table = block_table.size(1) > 1 && block_table.stride(1) != 1
+        ? block_table.contiguous() : block_table;
+    const auto len = lengths.contiguous();
+
+    CacheArgs a = {};
+    a.q = qa.data_ptr();
+    a.cache = cache.data_ptr();
+    a.table = table.data_ptr<int>();
+    a.lengths = len.data_ptr<int>();
+    a.out = out.data_ptr();
+    a.q_b = qa.stride(0), a.q_s = qa.stride(1), a.q_h = qa.stride(2);
+    a.c_p = cache.stride(0), a.c_t = cache.stride(1);
+    a.t_b = table.stride(0);
+    a.pages = cache.size(0);
+    a.page_size = page;
+    a.page_shift = (page & (page - 1)) == 0 ? __builtin_ctzl(page) : -1;
+    a.page_of_groups = page % 8 == 0;
+    a.B = B, a.H = H, a.Sq = Sq, a.table_width = width;
+    a.rows = Sq * H;
+    a.scale = scale * 1.4426950408889634;
+    const int block_rows = a.rows <= 16 ? 16 : a.rows <= 32 ? 32
+                           : a.rows <= 64 ? 64 : 128;
+    a.row_groups = (a.rows + block_rows - 1) / block_rows;
+    // LDS holds one block a CU; no more blocks than there can be tiles
+    const int64_t items = B * a.row_groups;
+    const int64_t most = items * ((page * width + KEYS - 1) / KEYS);
+    const int blocks = std::min<int64_t>(256, most);
+    const int64_t slots = items + blocks;
+    auto part = torch::empty({slots * block_rows * (latent_dim + 2)},
+                             q.options().dtype(torch::kFloat));
+    a.part = part.data_ptr<float>();
+    a.part_stat = reinterpret_cast<float2*>(
+        a.part + slots * block_rows * latent_dim);
+    if (dtype == torch::kBFloat16)
+        cache_dispatch<__bf16>(a, latent_dim, rope, block_rows, blocks);
+    else
+        cache_dispatch<_Float16>(a, latent_dim, rope, block_rows, blocks);
+    HIP_CHECK_LAST();
+    return out;
+}

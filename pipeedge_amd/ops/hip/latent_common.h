@@ -1,24 +1,20 @@
 // Pieces shared by the two forms of latent attention: the swizzled LDS
 // images that LDS-DMA fills, their two kinds of fragment reads, and the
-// step from a score column in registers to the next product's operand.
+// running reference of the softmax.
 #pragma once
 
 #include "common.h"
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef unsigned uint2_ __attribute__((ext_vector_type(2)));
-typedef unsigned uint4_ __attribute__((ext_vector_type(4)));
 
 template <typename T> struct LatentVec;
 template <> struct LatentVec<__bf16> {
     typedef __bf16 v8 __attribute__((ext_vector_type(8)));
     typedef __bf16 v4 __attribute__((ext_vector_type(4)));
-    typedef __bf16 v2 __attribute__((ext_vector_type(2)));
 };
 template <> struct LatentVec<_Float16> {
     typedef _Float16 v8 __attribute__((ext_vector_type(8)));
     typedef _Float16 v4 __attribute__((ext_vector_type(4)));
-    typedef _Float16 v2 __attribute__((ext_vector_type(2)));
 };
 
 __device__ __forceinline__ f32x16 latent_mfma(LatentVec<__bf16>::v8 a,
@@ -32,20 +28,32 @@ __device__ __forceinline__ f32x16 latent_mfma(LatentVec<_Float16>::v8 a,
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
 
+__device__ __forceinline__ f32x4 latent_mfma(LatentVec<__bf16>::v8 a,
+                                             LatentVec<__bf16>::v8 b,
+                                             f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 latent_mfma(LatentVec<_Float16>::v8 a,
+                                             LatentVec<_Float16>::v8 b,
+                                             f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
 // An LDS image holds rows (tokens) of CH 16-byte chunks without padding, as
 // LDS-DMA writes it; chunk c of row r lies at chunk position c ^ key(r). The
-// key makes both reads free of bank conflicts (64 banks of 4 B):
+// key makes both reads free of bank conflicts (64 banks of 4 B; 256 B, 16 or
+// 32 lanes, a cycle):
 // - 16 consecutive rows at one chunk (the score product's operand),
-// - 4 consecutive rows at 4 adjacent chunks (the transposing reads of the
-//   value product).
-// Rows of 16k chunks all start at bank 0, so 16 keys are needed and rows
-// that differ in their low two bits go to different groups of 4 chunks; rows
-// of 16k + 8 chunks alternate between two halves already, rows of 8k + 4
-// between four quarters.
+// - 4 or 8 consecutive rows at 2 or 4 adjacent chunks (the transposing reads
+//   of the value product).
+// Rows of 16k chunks all start at bank 0, so 16 keys are needed: the low two
+// bits of the row choose among groups of 4 chunks, the third among pairs.
+// Rows of 16k + 8 chunks alternate between two halves already, rows of
+// 8k + 4 between four quarters.
 template <int CH>
 __device__ __forceinline__ constexpr int latent_key(int row) {
     if constexpr (CH % 16 == 0)
-        return ((row & 3) << 2) | ((row >> 2) & 3);
+        return ((row & 3) << 2) | (((row >> 2) & 1) << 1) | ((row >> 3) & 1);
     else if constexpr (CH % 8 == 0)
         return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
     else
@@ -67,62 +75,88 @@ __device__ __forceinline__ void latent_arrive() {
     asm volatile("" ::: "memory");
 }
 
-// chunk c of row r
-template <typename T, int CH>
+// Chunks that a key permutes among each other.
+template <int CH>
+__device__ __forceinline__ constexpr int latent_group() {
+    return CH % 16 == 0 ? 16 : CH % 8 == 0 ? 8 : 4;
+}
+
+// Fragment addresses are kept as one register a tile: a chunk number known
+// at compile time only flips address bits inside a group of chunks or adds a
+// constant, since rows and images begin at multiples of a group.
+
+__device__ __forceinline__ unsigned latent_lds(const void* p) {
+    return (unsigned)reinterpret_cast<uintptr_t>(p);    // byte address
+}
+
+// Both products run on M x M MFMAs, M = 16 (k = 32) or 32 (k = 16); the 64
+// lanes are 64 / M groups of M, and lane l gives k = 8 (l / M) + 0..7 of
+// row l % M.
+
+// Score operand: chunks (64 / M) i + l / M of row row0 + l % M
+template <int CH, int M>
+__device__ __forceinline__ unsigned latent_row_base(unsigned image,
+                                                    int lane) {
+    const int row = lane % M;
+    return image + row * CH * 16 + (((lane / M) ^ latent_key<CH>(row)) << 4);
+}
+template <typename T, int CH, int M>
 __device__ __forceinline__ typename LatentVec<T>::v8 latent_row_read(
-        const T* image, int row, int chunk) {
-    return *reinterpret_cast<const typename LatentVec<T>::v8*>(
-        image + (row * CH + (chunk ^ latent_key<CH>(row))) * 8);
+        unsigned base, int row0, int i) {
+    constexpr int G = latent_group<CH>(), STEP = 64 / M;
+    const unsigned at = (base ^ ((STEP * i % G) << 4))
+                        + (STEP * i / G) * G * 16 + row0 * CH * 16;
+    return *reinterpret_cast<const __attribute__((address_space(3)))
+        typename LatentVec<T>::v8*>((uintptr_t)at);
 }
 
 template <typename T>
 __device__ __forceinline__ typename LatentVec<T>::v4 latent_tr_read(
-        const T* p) {
+        unsigned at) {
     typedef __attribute__((address_space(3))) LatentVec<__bf16>::v4 lds_v4;
     const auto r = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
-        reinterpret_cast<lds_v4*>(reinterpret_cast<uintptr_t>(p)));
+        reinterpret_cast<lds_v4*>((uintptr_t)at));
     return __builtin_bit_cast(typename LatentVec<T>::v4, r);
 }
 
-// A-operand of the value product, V^T[32 columns from col0][16 tokens from
-// row0]: lane l gets column l & 31 of tokens row0 + (l >> 5) * 8 + 0..7. A
-// transposing read turns 4 rows of 16 columns, given as 4 adjacent elements
-// by each of 16 lanes, into one column of 4 rows for each of them.
-template <typename T, int CH>
+// Value operand, V^T[M columns from M n][tokens]: lane l gets column l % M.
+// The sum over tokens may take them in any order, so the 8 values of a lane
+// are those tokens whose scores the lane holds: 4 (l / M) + 0..3 and the same
+// + 256 / M, counted from row0. No weight ever crosses lanes. A transposing
+// read turns 4 rows of 16 columns, given as 4 adjacent elements by each of 16
+// lanes, into one column of 4 rows for each of them.
+template <int CH, int M>
+__device__ __forceinline__ unsigned latent_column_base(unsigned image,
+                                                       int lane) {
+    const int row = lane / M * 4 + ((lane & 15) >> 2);
+    const int chunk = (lane % M >= 16 ? 2 : 0) + ((lane & 3) >> 1);
+    return image + row * CH * 16 + ((chunk ^ latent_key<CH>(row)) << 4)
+           + (lane & 1) * 8;
+}
+template <typename T, int CH, int M>
 __device__ __forceinline__ typename LatentVec<T>::v8 latent_column_read(
-        const T* image, int row0, int col0, int lane) {
-    const int row = row0 + (lane >> 5) * 8 + ((lane & 15) >> 2);
-    const int col = col0 + (lane & 16) + (lane & 3) * 4;
-    const auto at = [&](int r) {
-        return image + (r * CH + ((col >> 3) ^ latent_key<CH>(r))) * 8
-               + (col & 7);
-    };
-    const auto lo = latent_tr_read<T>(at(row));
-    const auto hi = latent_tr_read<T>(at(row + 4));
+        unsigned base, int row0, int n) {
+    constexpr int G = latent_group<CH>(), STEP = M / 8;
+    constexpr int NEXT = 256 / M;       // rows to the second read
+    // 16 rows on, a row's key is the same; 8 rows on, one bit differs
+    constexpr unsigned flip8 =
+        NEXT == 16 ? 0 : (latent_key<CH>(8) ^ latent_key<CH>(0)) << 4;
+    const unsigned flip = (STEP * n % G) << 4;
+    const unsigned add = (STEP * n / G) * G * 16 + row0 * CH * 16;
+    const auto lo = latent_tr_read<T>((base ^ flip) + add);
+    const auto hi = latent_tr_read<T>((base ^ flip ^ flip8) + add
+                                      + NEXT * CH * 16);
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-template <typename T>
-__device__ __forceinline__ unsigned latent_pack(float lo, float hi) {
-    typename LatentVec<T>::v2 v = {(T)lo, (T)hi};
-    return __builtin_bit_cast(unsigned, v);
-}
-
-// B-operand of the value product for tokens 16c .. 16c+15 of a 32-token
-// score column: a lane's scores are tokens (lane >> 5) * 4 + 8 * (i >> 2) +
-// (i & 3), the operand wants (lane >> 5) * 8 + 0..7, so the two halves of
-// the wave exchange four values each.
+// eight weights, rounded to the type of the values they multiply
 template <typename T>
 __device__ __forceinline__ typename LatentVec<T>::v8 latent_weights(
-        const f32x16& p, int c) {
-    const unsigned u0 = latent_pack<T>(p[8 * c + 0], p[8 * c + 1]);
-    const unsigned u1 = latent_pack<T>(p[8 * c + 2], p[8 * c + 3]);
-    const unsigned v0 = latent_pack<T>(p[8 * c + 4], p[8 * c + 5]);
-    const unsigned v1 = latent_pack<T>(p[8 * c + 6], p[8 * c + 7]);
-    const uint2_ w0 = __builtin_amdgcn_permlane32_swap(u0, v0, false, false);
-    const uint2_ w1 = __builtin_amdgcn_permlane32_swap(u1, v1, false, false);
-    const uint4_ w = {w0.x, w1.x, w0.y, w1.y};
-    return __builtin_bit_cast(typename LatentVec<T>::v8, w);
+        const float (&w)[8]) {
+    typename LatentVec<T>::v8 r;
+    #pragma unroll
+    for (int j = 0; j < 8; ++j) r[j] = (T)w[j];
+    return r;
 }
 
 // Running reference of the softmax, in powers of two. Weights are kept as

@@ -261,3 +261,61 @@ def latent_attention(q: Tensor, kv: Tensor, k_rope: Tensor, scale: float,
     weight = _softmax_seen(scores, seen.unsqueeze(1))
     out = torch.matmul(weight, heads[..., nope:].contiguous())
     return out.transpose(1, 2).contiguous().to(q.dtype)
+
+
+def check_latent_cache_attention(q: Tensor, cache: Tensor,
+                                 block_table: Tensor, lengths: Tensor,
+                                 latent_dim: int, scale: float):
+    """The argument checks of the latent cache kernel (CPU path)."""
+    op = "latent_cache_attention"
+    if q.dtype != cache.dtype:
+        raise TypeError(f"{op}: q and cache must have one type")
+    if block_table.dtype != torch.int32 or lengths.dtype != torch.int32:
+        raise TypeError(f"{op}: block_table and lengths must be int32")
+    if any(t.device != q.device for t in (cache, block_table, lengths)):
+        raise ValueError(f"{op}: tensors on different devices")
+    _check_inference(op, q, cache)
+    if q.dim() != 4 or cache.dim() != 3 or q.shape[3] != cache.shape[2]:
+        raise ValueError(f"{op}: q must be [B, Sq, H, D] and cache [pages, "
+                         f"page size, D], got {list(q.shape)} and "
+                         f"{list(cache.shape)}")
+    b, rope = q.shape[0], q.shape[3] - latent_dim
+    if latent_dim not in (256, 512) or rope not in (32, 64):
+        raise ValueError(f"{op}: rows must be 256 or 512 latent and 32 or 64 "
+                         f"rotary columns, got {latent_dim} and {rope}")
+    if block_table.dim() != 2 or block_table.shape[0] != b \
+            or lengths.shape != (b,):
+        raise ValueError(f"{op}: block_table must be [B, P] and lengths [B]")
+    if not 0.0 < scale < math.inf:
+        raise ValueError(f"{op}: scale must be positive")
+
+
+def latent_cache_attention(q: Tensor, cache: Tensor, block_table: Tensor,
+                           lengths: Tensor, latent_dim: int,
+                           scale: float) -> Tensor:
+    """Every head of the last ``Sq`` tokens attends to the cached rows, whose
+    first ``latent_dim`` columns are also the values."""
+    check_latent_cache_attention(q, cache, block_table, lengths, latent_dim,
+                                 scale)
+    b, sq, h, width = q.shape
+    page = cache.shape[1]
+    out = q.new_zeros(b, sq, h, latent_dim)
+    for i in range(b):
+        n = int(lengths[i])
+        if n <= 0 or out.numel() == 0:
+            continue
+        place = torch.arange(n, device=q.device)
+        if page == 0 or n > page * block_table.shape[1]:
+            out[i] = float("nan")
+            continue
+        pages = block_table[i].long()[place // page]
+        if ((pages < 0) | (pages >= cache.shape[0])).any():
+            out[i] = float("nan")
+            continue
+        tokens = cache[pages, place % page].float()
+        scores = torch.matmul(q[i].float().contiguous(), tokens.t()) * scale
+        at = n - sq + torch.arange(sq, device=q.device)
+        seen = place <= at.reshape(sq, 1, 1)
+        weight = _softmax_seen(scores, seen.expand(sq, h, n))
+        out[i] = torch.matmul(weight, tokens[:, :latent_dim]).to(q.dtype)
+    return out

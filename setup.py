@@ -27,6 +27,7 @@ ext = CUDAExtension(
         os.path.join(HIP_DIR, "quantpack.hip"),
         os.path.join(HIP_DIR, "rotary.hip"),
         os.path.join(HIP_DIR, "latent_attention.hip"),
+        os.path.join(HIP_DIR, "latent_cache.hip"),
         os.path.join(HIP_DIR, "debug_probe.hip"),
     ],
     extra_compile_args={

@@ -225,3 +225,237 @@ def test_expanded_graph():
         torch.cuda.synchronize()
         want = ops.latent_attention(q, kv, k_rope, causal=True, lengths=n)
         assert torch.equal(out, want)
+
+
+# ---------------------------------------------------------------- absorbed
+
+def cache_exact(q, cache, table, lengths, latent, scale):
+    b, sq, h, width = q.shape
+    q, cache, table = q.cpu(), cache.cpu(), table.cpu().long()
+    page = cache.shape[1]
+    ref = torch.zeros(b, sq, h, latent, dtype=torch.float64)
+    size, drift = torch.zeros_like(ref), torch.zeros(b, sq, h).double()
+    for i in range(b):
+        n = int(lengths[i])
+        if n == 0:
+            continue
+        place = torch.arange(n)
+        tokens = cache[table[i, place // page], place % page]
+        upto = (n - sq + 1 + torch.arange(sq)).clamp(min=0)
+        r, s, d = attend(q[i].reshape(sq * h, width), tokens,
+                         tokens[:, :latent], scale,
+                         upto.repeat_interleave(h))
+        ref[i], size[i] = r.view(sq, h, latent), s.view(sq, h, latent)
+        drift[i] = d.view(sq, h)
+    return ref, size, drift
+
+
+def make_cache(lengths, sq, h, latent, rope, page, dtype, device, seed=0,
+               spare=2):
+    """Pages in random order; unused table entries and the rows behind each
+    sequence's last hold what must never be read or used."""
+    torch.manual_seed(seed + sq + h)
+    b, width = len(lengths), latent + rope
+    counts = [-(-n // page) for n in lengths]
+    pages = sum(counts) + spare
+    cache = torch.full((pages, page, width), float("nan"))
+    order = torch.randperm(pages).tolist()
+    table = torch.full((b, max(max(counts), 1) + 1), -12345,
+                       dtype=torch.int32)
+    at = 0
+    for i, n in enumerate(lengths):
+        for j in range(counts[i]):
+            table[i, j] = order[at]
+            rows = min(page, n - j * page)
+            cache[order[at], :rows] = torch.randn(rows, width)
+            at += 1
+    q = torch.randn(b, sq, h, width)
+    return (q.to(dtype).to(device), cache.to(dtype).to(device),
+            table.to(device),
+            torch.tensor(lengths, dtype=torch.int32, device=device))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("latent,rope,page", [
+    (512, 64, 64), (512, 32, 16), (256, 64, 8), (256, 32, 1),
+    (512, 64, 24), (256, 64, 7), (512, 32, 3),
+])
+@pytest.mark.parametrize("sq,h,lengths", [
+    (1, 1, [1]),
+    (1, 16, [517, 1, 64, 0, 63, 65, 300]),
+    (1, 20, [100, 33, 0, 257]),
+    (3, 12, [2, 31, 190, 1, 0]),     # queries before the start
+    (2, 64, [129, 400]),             # a full block of rows
+    (3, 50, [77, 5]),                # two blocks of rows, the last ragged
+])
+def test_cache_matches_exact(device, dtype, latent, rope, page, sq, h,
+                             lengths):
+    q, cache, table, n = make_cache(lengths, sq, h, latent, rope, page, dtype,
+                                    device)
+    out = ops.latent_cache_attention(q, cache, table, n, latent_dim=latent,
+                                     scale=0.07)
+    assert out.shape == (len(lengths), sq, h, latent) and out.dtype == dtype
+    check(out, *cache_exact(q, cache, table, lengths, latent, 0.07), dtype)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_cache_long_and_many(device):
+    """Runs of tiles that cross sequences, and more sequences than a wave."""
+    lengths = [(37 * i) % 200 for i in range(150)] + [5000, 0, 3]
+    q, cache, table, n = make_cache(lengths, 1, 4, 256, 32, 16,
+                                    torch.bfloat16, device)
+    out = ops.latent_cache_attention(q, cache, table, n, latent_dim=256,
+                                     scale=0.07)
+    check(out, *cache_exact(q, cache, table, lengths, 256, 0.07),
+          torch.bfloat16)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_cache_peaked_scores(device, dtype):
+    """Scores that rise along the cache move the reference in every tile."""
+    lengths = [700, 900]
+    q, cache, table, n = make_cache(lengths, 1, 16, 256, 32, 64, dtype,
+                                    device)
+    q[..., 0] = 4.0
+    for i, length in enumerate(lengths):
+        place = torch.arange(length, device=device)
+        cache[table[i].long()[place // 64], place % 64, 0] = torch.linspace(
+            -30, 30, length, device=device).to(dtype)
+    out = ops.latent_cache_attention(q, cache, table, n, latent_dim=256,
+                                     scale=0.5)
+    check(out, *cache_exact(q, cache, table, lengths, 256, 0.5), dtype)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_cache_strided(device):
+    """A layer's slice of a larger cache, queries with heads first, a table
+    that is part of a wider one."""
+    lengths = [130, 64, 17]
+    q, cache, table, n = make_cache(lengths, 2, 6, 256, 64, 16,
+                                    torch.float16, device)
+    want = ops.latent_cache_attention(q, cache, table, n, latent_dim=256,
+                                      scale=0.1)
+    layers = torch.zeros(cache.shape[0], 3, 16, 320, dtype=cache.dtype,
+                         device=device)
+    layers[:, 1] = cache
+    by_token = torch.zeros(cache.shape[0], 16, 2, 336, dtype=cache.dtype,
+                           device=device)
+    by_token[:, :, 1, 16:] = cache
+    q2 = q.transpose(1, 2).contiguous().transpose(1, 2)
+    wide = torch.zeros(3, table.shape[1] * 2, dtype=torch.int32,
+                       device=device)
+    wide[:, 1::2] = table
+    for c in (layers[:, 1], by_token[:, :, 1, 16:]):
+        for t in (table, wide[:, 1::2]):
+            got = ops.latent_cache_attention(q2, c, t, n, latent_dim=256,
+                                             scale=0.1)
+            assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_cache_bad_pages_and_lengths(device):
+    """They spoil their own sequence and no other. On the CPU first: the GPU
+    run follows where the reference is clear."""
+    lengths = [130, 64, 17, 40]
+    args = (lengths, 1, 4, 256, 32, 16, torch.bfloat16, device)
+    q, cache, table, n = make_cache(*args)
+    good = ops.latent_cache_attention(q, cache, table, n, latent_dim=256,
+                                      scale=0.1)
+    assert torch.isfinite(good).all()
+    for page in (-1, cache.shape[0], 2 ** 31 - 1, -2 ** 31):
+        t = table.clone()
+        t[0, 3] = page
+        t[2, 0] = page
+        out = ops.latent_cache_attention(q, cache, t, n, latent_dim=256,
+                                         scale=0.1)
+        assert torch.isnan(out[0]).all() and torch.isnan(out[2]).all()
+        assert torch.equal(out[1], good[1]) and torch.equal(out[3], good[3])
+    m = n.clone()
+    m[1] = table.shape[1] * 16 + 1
+    t = table.clone()
+    t[1] = 0
+    out = ops.latent_cache_attention(q, cache, t, m, latent_dim=256,
+                                     scale=0.1)
+    assert torch.isnan(out[1]).all()
+    assert torch.equal(out[0], good[0]) and torch.equal(out[2:], good[2:])
+    m[1] = -5
+    out = ops.latent_cache_attention(q, cache, t, m, latent_dim=256,
+                                     scale=0.1)
+    assert not out[1].any() and torch.equal(out[0], good[0])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_cache_empty(device):
+    q, cache, table, n = make_cache([5, 3], 1, 4, 256, 32, 16,
+                                    torch.bfloat16, device)
+    kw = dict(latent_dim=256, scale=0.1)
+    for x in (q[:, :0], q[:, :, :0]):
+        assert ops.latent_cache_attention(
+            x, cache, table, n, **kw).shape == x.shape[:3] + (256,)
+    assert ops.latent_cache_attention(q[:0], cache, table[:0], n[:0],
+                                      **kw).shape == (0, 1, 4, 256)
+    out = ops.latent_cache_attention(q, cache, table[:, :0], n * 0, **kw)
+    assert not out.any()
+    out = ops.latent_cache_attention(q, cache, table[:, :0], n, **kw)
+    assert torch.isnan(out).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_cache_refusals(device):
+    q, cache, table, n = make_cache([5, 3], 1, 4, 256, 32, 16,
+                                    torch.bfloat16, device)
+    kw = dict(latent_dim=256, scale=0.1)
+    bad = [
+        ((q.half(), cache, table, n), kw), ((q[0], cache, table, n), kw),
+        ((q, cache[0], table, n), kw), ((q[..., :280], cache, table, n), kw),
+        ((q, cache, table.long(), n), kw), ((q, cache, table, n.long()), kw),
+        ((q, cache, table[:1], n), kw), ((q, cache, table, n[:1]), kw),
+        ((q, cache, table[0], n), kw),
+        ((q, cache, table, n), dict(latent_dim=240, scale=0.1)),
+        ((q, cache, table, n), dict(latent_dim=288, scale=0.1)),
+        ((q, cache, table, n), dict(latent_dim=256, scale=-1.0)),
+        ((q.clone().requires_grad_(), cache, table, n), kw),
+    ]
+    for args, k in bad:
+        with pytest.raises((TypeError, ValueError)):
+            ops.latent_cache_attention(*args, **k)
+    if device == "cuda":
+        odd = torch.zeros(3, 16, 292, dtype=q.dtype, device=device)[..., 4:]
+        for c in (odd, cache.cpu(), cache[:0],
+                  cache.transpose(1, 2).contiguous().transpose(1, 2)):
+            with pytest.raises(ValueError):
+                ops.latent_cache_attention(q, c, table, n, **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("h", [4, 16, 40, 128])
+def test_cache_graph_and_repeats(h):
+    """Replays with other lengths and caches equal the eager call, and so do
+    two graphs on two streams at once."""
+    lengths = [900, 40, 333, 0]
+    q, cache, table, n = make_cache(lengths, 1, h, 256, 64, 16,
+                                    torch.bfloat16, "cuda")
+    cache = torch.nan_to_num(cache)
+    table = table.clamp(min=0)
+    kw = dict(latent_dim=256, scale=0.1)
+    ops.latent_cache_attention(q, cache, table, n, **kw)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(ops.latent_cache_attention(q, cache, table, n, **kw))
+        graphs.append(g)
+    side = torch.cuda.Stream()
+    for i in range(3):
+        cache.copy_(torch.randn_like(cache))
+        n.copy_(torch.tensor([900 - 300 * i, 1 + i, 320, 64 * i]))
+        want = ops.latent_cache_attention(q, cache, table, n, **kw)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            graphs[1].replay()
+        graphs[0].replay()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want) and torch.equal(outs[1], want)
