@@ -298,3 +298,27 @@ def latent_cache_attention(q: Tensor, cache: Tensor, block_table: Tensor,
     run = _hip.latent_cache_attention if _use_hip(q) \
         else torch_ref.latent_cache_attention
     return run(q, cache, block_table, lengths, latent_dim, scale)
+
+
+def adapter_linear(x: Tensor, weight_nk: Tensor, down: Tensor, up: Tensor,
+                   ids: Tensor, bias: Optional[Tensor] = None,
+                   act: Optional[str] = None,
+                   residual: Optional[Tensor] = None,
+                   scales: Optional[Tensor] = None) -> Tensor:
+    """``linear`` beside low-rank adapters of many requests, for a batch whose
+    items belong to different tenants of one set of weights:
+
+      y = act(x W^T + bias + scales[i] (x down[i]^T) up[i]^T) + residual
+
+    ``down`` [n, r, K] and ``up`` [n, N, r] stack the adapters (r <= 256);
+    ``ids`` (int32) gives each item of the batch ([B]) or each row
+    (x.shape[:-1]) its adapter, and any value outside 0 .. n-1, such as -1,
+    none. ``scales`` (float32 [n]) defaults to ones. bfloat16 on the GPU. A
+    row is touched by no adapter but its own, whatever the others hold."""
+    if act not in _ACT_CODE:
+        raise ValueError(f"unknown activation: {act}")
+    if _use_hip(x):
+        return _hip.adapter_linear(x, weight_nk, down, up, ids, bias,
+                                   _ACT_CODE[act], residual, scales)
+    return torch_ref.adapter_linear(x, weight_nk, down, up, ids, bias, act,
+                                    residual, scales)

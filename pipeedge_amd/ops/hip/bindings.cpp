@@ -4,6 +4,8 @@
 // every GPU tensor; there is no eager fallback on GPU (fail-loud contract).
 #include <torch/extension.h>
 
+#include "adapter.h"
+
 std::tuple<torch::Tensor, torch::Tensor> gemm_bf16(
         torch::Tensor a2d, torch::Tensor b,
         c10::optional<torch::Tensor> bias, int64_t act,
@@ -11,7 +13,8 @@ std::tuple<torch::Tensor, torch::Tensor> gemm_bf16(
         c10::optional<torch::Tensor> ln_stats = c10::nullopt,
         c10::optional<torch::Tensor> ln_s = c10::nullopt,
         c10::optional<torch::Tensor> ln_c = c10::nullopt,
-        double ln_eps = 1e-12, bool want_stats = false);
+        double ln_eps = 1e-12, bool want_stats = false,
+        const AdapterRows* adapters = nullptr);
 torch::Tensor ln_stats_bf16(torch::Tensor x);
 torch::Tensor debug_mfma_tile(torch::Tensor a, torch::Tensor b);
 torch::Tensor layernorm_bf16(torch::Tensor x, torch::Tensor weight,
@@ -44,6 +47,12 @@ torch::Tensor latent_attention_op(
 torch::Tensor latent_cache_attention_op(
         torch::Tensor q, torch::Tensor cache, torch::Tensor block_table,
         torch::Tensor lengths, int64_t latent_dim, double scale);
+torch::Tensor adapter_linear_op(
+        torch::Tensor x, torch::Tensor weight, torch::Tensor down,
+        torch::Tensor up, torch::Tensor ids,
+        c10::optional<torch::Tensor> bias, int64_t act,
+        c10::optional<torch::Tensor> residual,
+        c10::optional<torch::Tensor> scales);
 
 namespace {
 
@@ -121,6 +130,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("latent_cache_attention", &latent_cache_attention_op, py::arg("q"),
           py::arg("cache"), py::arg("block_table"), py::arg("lengths"),
           py::arg("latent_dim"), py::arg("scale"));
+    m.def("adapter_linear", &adapter_linear_op, py::arg("x"),
+          py::arg("weight"), py::arg("down"), py::arg("up"), py::arg("ids"),
+          py::arg("bias") = py::none(), py::arg("act") = 0,
+          py::arg("residual") = py::none(), py::arg("scales") = py::none());
     m.def("_debug_mfma_tile", &debug_mfma_tile);
     m.def("_debug_mfma32_raw", &debug_mfma32_raw);
     m.def("_debug_tr16_raw", &debug_tr16_raw);

@@ -319,3 +319,81 @@ def latent_cache_attention(q: Tensor, cache: Tensor, block_table: Tensor,
         weight = _softmax_seen(scores, seen.expand(sq, h, n))
         out[i] = torch.matmul(weight, tokens[:, :latent_dim]).to(q.dtype)
     return out
+
+
+def check_adapter_linear(x: Tensor, weight: Tensor, down: Tensor, up: Tensor,
+                         ids: Tensor, bias: Optional[Tensor],
+                         residual: Optional[Tensor],
+                         scales: Optional[Tensor]):
+    """The argument checks of the adapter projection (CPU path)."""
+    op = "adapter_linear"
+    if any(t is not None and t.dtype != x.dtype
+           for t in (weight, down, up, bias, residual)):
+        raise TypeError(f"{op}: x, weight, down, up, bias and residual must "
+                        "have one type")
+    if ids.dtype != torch.int32:
+        raise TypeError(f"{op}: ids must be int32")
+    if scales is not None and scales.dtype != torch.float32:
+        raise TypeError(f"{op}: scales must be float32")
+    tensors = (weight, down, up, ids, bias, residual, scales)
+    if any(t is not None and t.device != x.device for t in tensors):
+        raise ValueError(f"{op}: tensors on different devices")
+    _check_inference(op, x, *tensors)
+    if x.dim() < 1 or weight.dim() != 2 or down.dim() != 3 or up.dim() != 3:
+        raise ValueError(f"{op}: x must be [.., K], weight [N, K], "
+                         "down [n, r, K] and up [n, N, r]")
+    n, r, k = down.shape
+    if x.shape[-1] != k or weight.shape[1] != k \
+            or up.shape != (n, weight.shape[0], r):
+        raise ValueError(f"{op}: x {list(x.shape)}, weight "
+                         f"{list(weight.shape)}, down {list(down.shape)} and "
+                         f"up {list(up.shape)} do not match")
+    if k == 0:
+        raise ValueError(f"{op}: no inner columns, or too many rows")
+    if r > 256:
+        raise ValueError(f"{op}: rank above 256")
+    if ids.shape != x.shape[:-1] and not (
+            x.dim() >= 2 and ids.shape == x.shape[:1]):
+        raise ValueError(f"{op}: ids must be one a row or one an item of the "
+                         f"batch, got {list(ids.shape)}")
+    if bias is not None and bias.shape != weight.shape[:1]:
+        raise ValueError(f"{op}: bias must be [N]")
+    if residual is not None \
+            and residual.shape != x.shape[:-1] + weight.shape[:1]:
+        raise ValueError(f"{op}: residual must have the output's shape")
+    if scales is not None and scales.shape != (n,):
+        raise ValueError(f"{op}: scales must be [n]")
+
+
+def adapter_linear(x: Tensor, weight: Tensor, down: Tensor, up: Tensor,
+                   ids: Tensor, bias: Optional[Tensor] = None,
+                   act: Optional[str] = None,
+                   residual: Optional[Tensor] = None,
+                   scales: Optional[Tensor] = None) -> Tensor:
+    """``linear`` plus ``scales[i] * (x @ down[i].T) @ up[i].T`` before the
+    activation, with i the row's id; ids outside the stack have no adapter."""
+    check_adapter_linear(x, weight, down, up, ids, bias, residual, scales)
+    rows = x.float().reshape(-1, x.shape[-1])
+    per = rows.shape[0] // max(ids.numel(), 1)
+    row_ids = ids.reshape(-1).repeat_interleave(per)
+    y = rows @ weight.float().t()
+    for i in row_ids.unique().tolist():
+        if not 0 <= i < down.shape[0]:
+            continue
+        mine = row_ids == i
+        inner = rows[mine] @ down[i].float().t()
+        if scales is not None:
+            inner = inner * scales[i]
+        y[mine] += inner @ up[i].float().t()
+    if bias is not None:
+        y = y + bias.float()
+    if act == "gelu":
+        y = torch.nn.functional.gelu(y)
+    elif act == "tanh":
+        y = torch.tanh(y)
+    elif act is not None:
+        raise ValueError(f"unknown activation: {act}")
+    y = y.reshape(*x.shape[:-1], weight.shape[0])
+    if residual is not None:
+        y = y + residual.float()
+    return y.to(x.dtype)

@@ -25,6 +25,7 @@ ext = CUDAExtension(
         os.path.join(HIP_DIR, "attention.hip"),
         os.path.join(HIP_DIR, "patchify.hip"),
         os.path.join(HIP_DIR, "quantpack.hip"),
+        os.path.join(HIP_DIR, "adapter.hip"),
         os.path.join(HIP_DIR, "rotary.hip"),
         os.path.join(HIP_DIR, "latent_attention.hip"),
         os.path.join(HIP_DIR, "latent_cache.hip"),

@@ -1,0 +1,219 @@
+"""The adapter projection against its definition in 64 bits. Every case runs
+on the CPU path; with a GPU the same cases run on the HIP kernels."""
+import pytest
+import torch
+
+from pipeedge_amd import ops
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+
+
+def make(shape, k, n, rank, count, device, seed=0):
+    torch.manual_seed(seed + k + n + rank)
+    x = torch.randn(*shape, k)
+    w = torch.randn(n, k) * k ** -0.5
+    down = torch.randn(count, rank, k) * k ** -0.5
+    up = torch.randn(count, n, rank) * 0.3
+    return [t.bfloat16().to(device) for t in (x, w, down, up)]
+
+
+def check(out, x, w, down, up, ids, bias=None, act=None, residual=None,
+          scales=None):
+    """Row by row. fp32 sums over K (k steps of the absolute products, for
+    the shared and the inner product), the inner values rounded to bf16 once
+    (half a step), fp32 sums over the rank, an activation of slope at most
+    1.13 that adds 2^-20, one rounding of the result."""
+    half = 2.0 ** -8
+    x, w, down, up, ids = (t.cpu() for t in (x, w, down, up, ids))
+    k = x.shape[-1]
+    rows = x.double().reshape(-1, k)
+    per = rows.shape[0] // max(ids.numel(), 1)
+    row_ids = ids.reshape(-1).repeat_interleave(per)
+    y = rows @ w.double().t()
+    bound = rows.abs() @ w.double().abs().t() * k * 2.0 ** -24
+    for i in range(down.shape[0]):
+        mine = row_ids == i
+        a, b = down[i].double(), up[i].double()
+        s = 1.0 if scales is None else float(scales[i])
+        inner = rows[mine] @ a.t() * s
+        slack = inner.abs() * half + (rows[mine].abs() @ a.abs().t()
+                                      * abs(s) * (k + 2) * 2.0 ** -24)
+        y[mine] += inner @ b.t()
+        bound[mine] += slack @ b.abs().t() + (
+            inner.abs() @ b.abs().t() * (b.shape[1] + 2) * 2.0 ** -24)
+    if bias is not None:
+        y = y + bias.cpu().double()
+    bound = bound + y.abs() * 4 * 2.0 ** -24
+    if act == "gelu":
+        y = y * torch.special.ndtr(y)
+    elif act == "tanh":
+        y = torch.tanh(y)
+    if act is not None:
+        bound = bound * 1.13 + 2.0 ** -20
+    if residual is not None:
+        y = y + residual.cpu().double().reshape(y.shape)
+    bound = bound + y.abs() * half + 1e-30
+    assert out.dtype == torch.bfloat16
+    err = (out.double().cpu().reshape(y.shape) - y).abs()
+    assert (err <= bound).all(), (err / bound).max()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("shape,k,n,rank,count", [
+    ((1, 1), 64, 16, 8, 1),
+    ((8, 1), 1024, 500, 16, 8),      # one row of each request
+    ((70, 1), 256, 130, 16, 70),
+    ((5, 13), 192, 257, 8, 3),       # requests that end inside a tile
+    ((3, 197), 128, 96, 64, 2),
+    ((4, 33), 72, 61, 3, 4),         # nothing a multiple of 8
+    ((2, 9), 37, 23, 5, 2),
+    ((2, 40), 320, 48, 100, 2),
+    ((2, 20), 64, 40, 256, 2),
+    ((9, 150), 2048, 70, 24, 3),     # the tiles of long rows
+    ((11, 197), 64, 3200, 16, 3),    # of many wide rows
+    ((8, 200), 128, 4100, 8, 3),
+    ((17, 197), 2048, 3100, 8, 5),
+])
+def test_adapter_matches_exact(device, shape, k, n, rank, count):
+    x, w, down, up = make(shape, k, n, rank, count, device)
+    ids = torch.randperm(shape[0]).int() % (count + 1) - 1
+    ids = ids.to(device)
+    scales = (torch.rand(count) + 0.5).to(device)
+    bias = torch.randn(n).bfloat16().to(device)
+    res = torch.randn(*shape, n).bfloat16().to(device)
+    args = (x, w, down, up, ids)
+    out = ops.adapter_linear(*args)
+    assert out.shape == shape + (n,)
+    check(out, *args)
+    for kw in (dict(bias=bias, scales=scales),
+               dict(bias=bias, act="gelu", residual=res, scales=scales),
+               dict(act="tanh")):
+        check(ops.adapter_linear(*args, **kw), *args, **kw)
+    # one id a row, the requests' rows mixed
+    ids = (torch.arange(shape[0] * shape[1]) * 7 % (count + 2) - 1).int()
+    ids = ids.reshape(shape).to(device)
+    check(ops.adapter_linear(x, w, down, up, ids, bias, scales=scales),
+          x, w, down, up, ids, bias=bias, scales=scales)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_adapter_ids_outside(device):
+    """Rows without an adapter get the plain projection, bit for bit."""
+    x, w, down, up = make((6, 21), 128, 192, 16, 2, device)
+    bias = torch.randn(192).bfloat16().to(device)
+    ids = torch.tensor([-1, 0, 2, 1, -2 ** 31, 2 ** 31 - 1],
+                       dtype=torch.int32, device=device)
+    out = ops.adapter_linear(x, w, down, up, ids, bias)
+    check(out, x, w, down, up, ids, bias=bias)
+    none = torch.full_like(ids, -1)
+    plain = ops.adapter_linear(x, w, down, up, none, bias)
+    for i in (0, 2, 4, 5):
+        assert torch.equal(out[i], plain[i])
+    if device == "cuda":
+        assert torch.equal(plain, ops.linear(x, w, bias))
+    for empty in (down[:0], up[:0]), (down[:, :0], up[..., :0]):
+        assert torch.equal(ops.adapter_linear(x, w, *empty, ids, bias), plain)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("shape", [(8, 1), (6, 21), (24, 5)])
+def test_adapter_isolation(device, shape):
+    """Another request's infinite or undefined adapter, scale or input
+    reaches no row but its own."""
+    x, w, down, up = make(shape, 128, 192, 16, 3, device)
+    scales = torch.ones(3, device=device)
+    ids = (torch.arange(shape[0]) % 4 - 1).int().to(device)
+    want = ops.adapter_linear(x, w, down, up, ids, scales=scales)
+    down[1, 3, 5] = float("inf")
+    up[1, 100] = float("nan")
+    up[1, 7, 2] = float("inf")
+    scales[2] = float("nan")
+    x[0, 0, 0] = float("inf")
+    out = ops.adapter_linear(x, w, down, up, ids, scales=scales)
+    for i in range(shape[0]):
+        if int(ids[i]) in (-1, 0):
+            keep = slice(1, None) if i == 0 else slice(None)
+            assert torch.equal(out[i, keep], want[i, keep])
+        else:
+            assert not torch.isfinite(out[i]).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_adapter_strides(device):
+    x, w, down, up = make((4, 10), 96, 80, 12, 3, device)
+    ids = torch.tensor([2, 0, -1, 1], dtype=torch.int32, device=device)
+    want = ops.adapter_linear(x, w, down, up, ids)
+
+    def spread(t, at):
+        wide = torch.zeros(*t.shape[:-1], t.shape[-1] + 7, dtype=t.dtype,
+                           device=device)
+        wide[..., at:at + t.shape[-1]] = t
+        return wide[..., at:at + t.shape[-1]]
+    got = ops.adapter_linear(spread(x, 3), spread(w, 1), spread(down, 5),
+                             spread(up, 7), ids.repeat_interleave(2)[::2])
+    assert torch.equal(got, want)
+    got = ops.adapter_linear(x.transpose(0, 1).contiguous().transpose(0, 1),
+                             w, down, up, ids)
+    assert torch.equal(got, want)
+    flat = ops.adapter_linear(x.reshape(-1, 96), w, down, up,
+                              ids.repeat_interleave(10))
+    assert torch.equal(flat.view_as(want), want)
+    one = ops.adapter_linear(x[1, 2], w, down, up, ids[1])
+    check(one, x[1, 2].unsqueeze(0), w, down, up, ids[1:2])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_adapter_empty(device):
+    x, w, down, up = make((2, 3), 64, 32, 8, 2, device)
+    ids = torch.zeros(2, dtype=torch.int32, device=device)
+    assert ops.adapter_linear(x[:, :0], w, down, up, ids).shape == (2, 0, 32)
+    assert ops.adapter_linear(x[:0], w, down, up, ids[:0]).shape == (0, 3, 32)
+    assert ops.adapter_linear(x, w[:0], down, up[:, :0], ids).shape \
+        == (2, 3, 0)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_adapter_refusals(device):
+    x, w, down, up = make((2, 3), 64, 32, 8, 2, device)
+    ids = torch.zeros(2, dtype=torch.int32, device=device)
+    good = dict(x=x, weight_nk=w, down=down, up=up, ids=ids)
+    big = torch.zeros(2, 257, 64, dtype=x.dtype, device=device)
+    bad = [
+        dict(x=x.half()), dict(weight_nk=w.float()), dict(ids=ids.long()),
+        dict(ids=ids[:1]), dict(ids=ids.unsqueeze(1)), dict(x=x[..., :32]),
+        dict(down=down[:1]), dict(up=up[:, :8]), dict(up=up[..., :4]),
+        dict(weight_nk=w[0]), dict(down=big, up=big.transpose(1, 2)[:, :32]),
+        dict(bias=w[0]), dict(bias=w[:, 0].float()), dict(residual=x),
+        dict(scales=torch.ones(3, device=device)),
+        dict(scales=torch.ones(2, device=device).half()),
+        dict(act="relu"), dict(x=x.clone().requires_grad_()),
+        dict(up=up.clone().requires_grad_()),
+    ]
+    ops.adapter_linear(**good)
+    for change in bad:
+        with pytest.raises((TypeError, ValueError)):
+            ops.adapter_linear(**{**good, **change})
+    with torch.no_grad():
+        ops.adapter_linear(**{**good, "x": x.clone().requires_grad_()})
+    if device == "cuda":
+        for name in ("weight_nk", "ids"):
+            with pytest.raises(ValueError):
+                ops.adapter_linear(**{**good, name: good[name].cpu()})
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(8, 1), (8, 197)])
+def test_adapter_graph(shape):
+    x, w, down, up = make(shape, 256, 320, 16, 4, "cuda")
+    ids = torch.zeros(shape[0], dtype=torch.int32, device="cuda")
+    ops.adapter_linear(x, w, down, up, ids)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.adapter_linear(x, w, down, up, ids)
+    for i in range(3):
+        x.copy_(torch.randn_like(x))
+        ids.copy_((torch.arange(shape[0]) + i) % 5 - 1)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, ops.adapter_linear(x, w, down, up, ids))
