@@ -108,9 +108,140 @@ __global__ __launch_bounds__(256) void adapter_inner_kernel(InnerArgs a) {
     }
 }
 
+// Few rows: a wave takes one row and 4 inner columns, a block 16 of them. The
+// matrix unit would be idle for want of rows; what counts is that all the
+// adapters' rows are on their way at once.
+__global__ __launch_bounds__(256) void adapter_inner_step_kernel(
+        InnerArgs a) {
+    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+    const int row = blockIdx.x, col0 = blockIdx.y * 16 + wid * 4;
+    int id = a.row_ids[row / a.rows_per_id];
+    float sum[4] = {};
+    if (id >= 0 && id < a.n_adapters) {
+        const __bf16* x = a.x + (long)row * a.K;
+        const __bf16* down = a.down + (long)id * a.rank * a.K;
+        const __bf16* d[4];
+        #pragma unroll
+        for (int c = 0; c < 4; ++c)
+            d[c] = down + (long)min(col0 + c, a.rank - 1) * a.K;
+        #pragma unroll 2
+        for (int k = lane * 8; k < a.K; k += 512) {
+            const bf16x8 xv = inner_load(x, k, a.K, a.vec);
+            #pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const bf16x8 dv = inner_load(d[c], k, a.K, a.vec);
+                #pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    sum[c] = fmaf(bf2f(xv[j]), bf2f(dv[j]), sum[c]);
+            }
+        }
+        const float scale = a.scales != nullptr ? a.scales[id] : 1.0f;
+        #pragma unroll
+        for (int c = 0; c < 4; ++c)
+            sum[c] = wave64_reduce(sum[c], SumOp()) * scale;
+    }
+    if (lane == 0)
+        #pragma unroll
+        for (int c = 0; c < 4; ++c)
+            a.inner[(long)row * a.rank_pad + col0 + c] =
+                f2bf(col0 + c < a.rank ? sum[c] : 0.0f);
+}
+
+// The whole projection of few rows. Bound by reading W: a block takes 16
+// columns and all rows, its waves a part of K each, so that 4096 columns are
+// on 256 CUs and every wave has its loads on the way before it needs one.
+// The adapters' products are a short dot product for each output.
+constexpr int STEP_WAVES = 4;
+
+template <int NM>               // groups of 16 rows
+__global__ __launch_bounds__(64 * STEP_WAVES) void adapter_step_kernel(
+        const __bf16* __restrict__ x, const __bf16* __restrict__ w,
+        const __bf16* __restrict__ bias, const __bf16* __restrict__ residual,
+        __bf16* __restrict__ out, AdapterRows ad, int M, int N, int K,
+        int act, bool vec) {
+    constexpr int DEPTH = 4;    // steps of 32 in flight
+    __shared__ float parts[STEP_WAVES][NM][16][17];
+    const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+    const int l15 = lane & 15, quad = lane >> 4;
+    const int col0 = blockIdx.x * 16;
+
+    const int steps = (K + 31) / 32;
+    const int first = wid * steps / STEP_WAVES;
+    const int last = (wid + 1) * steps / STEP_WAVES;
+    const __bf16* wp = w + (long)min(col0 + l15, N - 1) * K + quad * 8;
+    const __bf16* xp[NM];
+    #pragma unroll
+    for (int m = 0; m < NM; ++m)
+        xp[m] = x + (long)min(m * 16 + l15, M - 1) * K + quad * 8;
+    f32x4 acc[NM] = {};
+    for (int s0 = first; s0 < last; s0 += DEPTH) {
+        bf16x8 wv[DEPTH], xv[DEPTH][NM];
+        #pragma unroll
+        for (int s = 0; s < DEPTH; ++s) {
+            // behind the wave's part nothing is loaded
+            const int k = (s0 + s) * 32;
+            const int end = s0 + s < last ? K - quad * 8 : 0;
+            wv[s] = inner_load(wp, k, end, vec);
+            #pragma unroll
+            for (int m = 0; m < NM; ++m)
+                xv[s][m] = inner_load(xp[m], k, end, vec);
+        }
+        #pragma unroll
+        for (int s = 0; s < DEPTH; ++s)
+            #pragma unroll
+            for (int m = 0; m < NM; ++m)
+                acc[m] = mfma_16x16x32_bf16(wv[s], xv[s][m], acc[m]);
+    }
+    // lane: row m * 16 + l15, columns quad * 4 ..
+    #pragma unroll
+    for (int m = 0; m < NM; ++m)
+        #pragma unroll
+        for (int r = 0; r < 4; ++r)
+            parts[wid][m][l15][quad * 4 + r] = acc[m][r];
+    __syncthreads();
+    #pragma unroll
+    for (int o = tid; o < NM * 256; o += 64 * STEP_WAVES) {
+        const int row = o / 16, c = o % 16, col = col0 + c;
+        if (row >= M || col >= N) continue;
+        float v = 0.0f;
+        #pragma unroll
+        for (int p = 0; p < STEP_WAVES; ++p)
+            v += parts[p][row / 16][row % 16][c];
+        const int id = ad.row_ids[row / ad.rows_per_id];
+        if (id >= 0 && id < ad.n_adapters) {
+            const __bf16* in = reinterpret_cast<const __bf16*>(ad.inner)
+                               + (long)row * ad.rank_pad;
+            const __bf16* up = reinterpret_cast<const __bf16*>(ad.up)
+                               + ((long)id * N + col) * ad.rank;
+            for (int k = 0; k < ad.rank; k += 8) {
+                const bf16x8 a = inner_load(in, k, ad.rank_pad, true);
+                const bf16x8 b = inner_load(up, k, ad.rank,
+                                            ad.rank % 8 == 0);
+                #pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    v = fmaf(bf2f(a[j]), bf2f(b[j]), v);
+            }
+        }
+        if (bias != nullptr) v += bf2f(bias[col]);
+        if (act == ACT_GELU) v = gelu_f(v);
+        else if (act == ACT_TANH) v = tanhf(v);
+        if (residual != nullptr) v += bf2f(residual[(long)row * N + col]);
+        out[(long)row * N + col] = f2bf(v);
+    }
+}
+
+// Rows that the kernels for few rows take.
+constexpr int STEP_ROWS = 64;
+
 void adapter_inner(const InnerArgs& a) {
-    // columns a block: all of them up to 64, then 64 at a time
     const dim3 block(256);
+    if (a.M <= STEP_ROWS) {
+        hipLaunchKernelGGL(adapter_inner_step_kernel,
+                           dim3(a.M, a.rank_pad / 16), block, 0,
+                           pe_current_stream(), a);
+        return;
+    }
+    // columns a block: all of them up to 64, then 64 at a time
     const int rows = (a.M + 15) / 16;
     if (a.rank_pad <= 32)
         hipLaunchKernelGGL((adapter_inner_kernel<2>), dim3(rows, 1), block, 0,
@@ -119,6 +250,19 @@ void adapter_inner(const InnerArgs& a) {
         hipLaunchKernelGGL((adapter_inner_kernel<4>),
                            dim3(rows, (a.rank_pad + 63) / 64), block, 0,
                            pe_current_stream(), a);
+}
+
+template <int NM>
+void adapter_step(const torch::Tensor& x, const torch::Tensor& w,
+                  const __bf16* bias, const __bf16* residual,
+                  torch::Tensor& out, const AdapterRows& rows, int act) {
+    const int M = x.size(0), N = w.size(0), K = x.size(1);
+    hipLaunchKernelGGL((adapter_step_kernel<NM>), dim3((N + 15) / 16),
+                       dim3(64 * STEP_WAVES), 0, pe_current_stream(),
+                       reinterpret_cast<const __bf16*>(x.data_ptr()),
+                       reinterpret_cast<const __bf16*>(w.data_ptr()), bias,
+                       residual, reinterpret_cast<__bf16*>(out.data_ptr()),
+                       rows, M, N, K, act, K % 8 == 0);
 }
 
 torch::Tensor adapter_dense(const torch::Tensor& x) {
@@ -238,6 +382,21 @@ torch::Tensor adapter_linear_op(
     const AdapterRows rows = {inner.data_ptr(), up_c.data_ptr(),
                               ids_c.data_ptr<int>(), in.rows_per_id, (int)n,
                               (int)r, rank_pad};
+    if (M <= STEP_ROWS) {
+        auto out = torch::empty(out_sizes, x.options());
+        const auto pointer = [](c10::optional<torch::Tensor>& t) {
+            if (!t.has_value()) return (const __bf16*)nullptr;
+            t = t->contiguous();
+            return reinterpret_cast<const __bf16*>(t->data_ptr());
+        };
+        const auto* b = pointer(bias);
+        const auto* res = pointer(res2d);
+        if (M <= 16) adapter_step<1>(x2d, w, b, res, out, rows, act);
+        else if (M <= 32) adapter_step<2>(x2d, w, b, res, out, rows, act);
+        else adapter_step<4>(x2d, w, b, res, out, rows, act);
+        HIP_CHECK_LAST();
+        return out;
+    }
     return std::get<0>(gemm_bf16(x2d, w, bias, act, res2d, 0, c10::nullopt,
                                  c10::nullopt, c10::nullopt, 1e-12, false,
                                  &rows)).reshape(out_sizes);
