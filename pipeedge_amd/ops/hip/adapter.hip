@@ -1,27 +1,35 @@
 // Projection with low-rank adapters of many requests,
 //   y = act(x W^T + b + s_i (x A_i^T) B_i^T) + residual,   i = id of the row,
 // in two launches: the inner values s_i x A_i^T of all rows, and the shared
-// GEMM, which adds their products with B_i to its accumulators before its
-// epilogue (gemm.hip), so y is written once and W is read as without
-// adapters. The inner values are rounded to bf16 once, as the operand of the
-// second product; the sums before and after stay in fp32.
+// product, which adds theirs with B_i to its accumulators before bias and
+// activation, so y is written once and W is read as without adapters. The
+// inner values are rounded to bf16 once, as the operand of the second product;
+// the sums before and after stay in fp32.
 #include <torch/extension.h>
 
 #include <c10/core/DeviceGuard.h>
 
-#include "adapter.h"
 #include "common.h"
-
-std::tuple<torch::Tensor, torch::Tensor> gemm_bf16(
-        torch::Tensor a2d, torch::Tensor b,
-        c10::optional<torch::Tensor> bias, int64_t act,
-        c10::optional<torch::Tensor> residual2d, int64_t tile,
-        c10::optional<torch::Tensor> ln_stats,
-        c10::optional<torch::Tensor> ln_s,
-        c10::optional<torch::Tensor> ln_c, double ln_eps, bool want_stats,
-        const AdapterRows* adapters);
+#include "mfma_tiles.h"
 
 namespace {
+
+// Which rows belong to which adapter, and what the second product reads.
+struct AdapterRows {
+    const __bf16* inner;        // [M][rank_pad], zero behind rank
+    const __bf16* up;           // [n_adapters][N][rank]
+    const int* row_ids;         // one for rows_per_id rows each
+    int rows_per_id, n_adapters, rank, rank_pad;
+};
+
+struct ProductArgs {
+    const __bf16 *x, *w, *bias, *residual;
+    __bf16* out;
+    int M, N, K, act;
+    bool vec;                   // K a multiple of 8
+    int m_blocks, n_blocks;
+    AdapterRows ad;
+};
 
 struct InnerArgs {
     const __bf16* x;            // [M][K]
@@ -51,6 +59,7 @@ __device__ __forceinline__ bf16x8 inner_load(const __bf16* p, int k, int K,
 // LDS and rows keep those of their own adapter.
 template <int NC>
 __global__ __launch_bounds__(256) void adapter_inner_kernel(InnerArgs a) {
+    constexpr int DEPTH = 4;    // steps of 32 whose loads are on their way
     __shared__ float parts[4][NC][64][4];
     const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
     const int l15 = lane & 15, quad = lane >> 4;
@@ -70,16 +79,25 @@ __global__ __launch_bounds__(256) void adapter_inner_kernel(InnerArgs a) {
         const unsigned rows = (unsigned)__ballot(id == cur) >> (quad * 4);
         const __bf16* down = a.down + (long)cur * a.rank * a.K + quad * 8;
         f32x4 acc[NC] = {};
-        for (int s = first; s < last; ++s) {
-            const int k = s * 32;
-            const bf16x8 xa = inner_load(x, k, a.K - quad * 8, a.vec);
+        for (int s0 = first; s0 < last; s0 += DEPTH) {
+            bf16x8 xv[DEPTH], dv[DEPTH][NC];
             #pragma unroll
-            for (int n = 0; n < NC; ++n) {
-                const int c = min(col0 + n * 16 + l15, a.rank - 1);
-                acc[n] = mfma_16x16x32_bf16(
-                    xa, inner_load(down + (long)c * a.K, k,
-                                   a.K - quad * 8, a.vec), acc[n]);
+            for (int s = 0; s < DEPTH; ++s) {
+                const int k = (s0 + s) * 32;
+                const int end = s0 + s < last ? a.K - quad * 8 : 0;
+                xv[s] = inner_load(x, k, end, a.vec);
+                #pragma unroll
+                for (int n = 0; n < NC; ++n) {
+                    const int c = min(col0 + n * 16 + l15, a.rank - 1);
+                    dv[s][n] = inner_load(down + (long)c * a.K, k, end,
+                                          a.vec);
+                }
             }
+            #pragma unroll
+            for (int s = 0; s < DEPTH; ++s)
+                #pragma unroll
+                for (int n = 0; n < NC; ++n)
+                    acc[n] = mfma_16x16x32_bf16(xv[s], dv[s][n], acc[n]);
         }
         #pragma unroll
         for (int n = 0; n < NC; ++n)
@@ -91,18 +109,23 @@ __global__ __launch_bounds__(256) void adapter_inner_kernel(InnerArgs a) {
     for (int n = 0; n < NC; ++n)
         *reinterpret_cast<f32x4*>(parts[wid][n][lane]) = mine[n];
     __syncthreads();
-    for (int n = wid; n < NC; n += 4) {
+    // 16 columns a wave; the padding behind the last is written by the last
+    // block of columns
+    const int pad = blockIdx.y + 1 == gridDim.y ? a.rank_pad
+                                                : col0 + 16 * NC;
+    for (int n = wid; col0 + n * 16 < pad; n += 4) {
         const int col = col0 + n * 16 + l15;
-        if (col >= a.rank_pad) continue;
         #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int out_row = row0 + quad * 4 + r;
             const int out_id = __shfl(id, quad * 4 + r);
             if (out_row >= a.M) continue;
-            float v = parts[0][n][lane][r] + parts[1][n][lane][r]
-                      + parts[2][n][lane][r] + parts[3][n][lane][r];
-            if (a.scales != nullptr && out_id >= 0) v *= a.scales[out_id];
-            if (out_id < 0 || col >= a.rank) v = 0.0f;
+            float v = 0.0f;
+            if (n < NC && col < a.rank && out_id >= 0) {
+                v = parts[0][n][lane][r] + parts[1][n][lane][r]
+                    + parts[2][n][lane][r] + parts[3][n][lane][r];
+                if (a.scales != nullptr) v *= a.scales[out_id];
+            }
             a.inner[(long)out_row * a.rank_pad + col] = f2bf(v);
         }
     }
@@ -155,10 +178,9 @@ constexpr int STEP_WAVES = 4;
 
 template <int NM>               // groups of 16 rows
 __global__ __launch_bounds__(64 * STEP_WAVES) void adapter_step_kernel(
-        const __bf16* __restrict__ x, const __bf16* __restrict__ w,
-        const __bf16* __restrict__ bias, const __bf16* __restrict__ residual,
-        __bf16* __restrict__ out, AdapterRows ad, int M, int N, int K,
-        int act, bool vec) {
+        ProductArgs a) {
+    const int M = a.M, N = a.N, K = a.K;
+    const AdapterRows& ad = a.ad;
     constexpr int DEPTH = 4;    // steps of 32 in flight
     __shared__ float parts[STEP_WAVES][NM][16][17];
     const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
@@ -168,11 +190,11 @@ __global__ __launch_bounds__(64 * STEP_WAVES) void adapter_step_kernel(
     const int steps = (K + 31) / 32;
     const int first = wid * steps / STEP_WAVES;
     const int last = (wid + 1) * steps / STEP_WAVES;
-    const __bf16* wp = w + (long)min(col0 + l15, N - 1) * K + quad * 8;
+    const __bf16* wp = a.w + (long)min(col0 + l15, N - 1) * K + quad * 8;
     const __bf16* xp[NM];
     #pragma unroll
     for (int m = 0; m < NM; ++m)
-        xp[m] = x + (long)min(m * 16 + l15, M - 1) * K + quad * 8;
+        xp[m] = a.x + (long)min(m * 16 + l15, M - 1) * K + quad * 8;
     f32x4 acc[NM] = {};
     for (int s0 = first; s0 < last; s0 += DEPTH) {
         bf16x8 wv[DEPTH], xv[DEPTH][NM];
@@ -181,10 +203,10 @@ __global__ __launch_bounds__(64 * STEP_WAVES) void adapter_step_kernel(
             // behind the wave's part nothing is loaded
             const int k = (s0 + s) * 32;
             const int end = s0 + s < last ? K - quad * 8 : 0;
-            wv[s] = inner_load(wp, k, end, vec);
+            wv[s] = inner_load(wp, k, end, a.vec);
             #pragma unroll
             for (int m = 0; m < NM; ++m)
-                xv[s][m] = inner_load(xp[m], k, end, vec);
+                xv[s][m] = inner_load(xp[m], k, end, a.vec);
         }
         #pragma unroll
         for (int s = 0; s < DEPTH; ++s)
@@ -209,25 +231,374 @@ __global__ __launch_bounds__(64 * STEP_WAVES) void adapter_step_kernel(
             v += parts[p][row / 16][row % 16][c];
         const int id = ad.row_ids[row / ad.rows_per_id];
         if (id >= 0 && id < ad.n_adapters) {
-            const __bf16* in = reinterpret_cast<const __bf16*>(ad.inner)
-                               + (long)row * ad.rank_pad;
-            const __bf16* up = reinterpret_cast<const __bf16*>(ad.up)
-                               + ((long)id * N + col) * ad.rank;
+            const __bf16* in = ad.inner + (long)row * ad.rank_pad;
+            const __bf16* up = ad.up + ((long)id * N + col) * ad.rank;
             for (int k = 0; k < ad.rank; k += 8) {
-                const bf16x8 a = inner_load(in, k, ad.rank_pad, true);
-                const bf16x8 b = inner_load(up, k, ad.rank,
+                const bf16x8 av = inner_load(in, k, ad.rank_pad, true);
+                const bf16x8 bv = inner_load(up, k, ad.rank,
                                             ad.rank % 8 == 0);
                 #pragma unroll
                 for (int j = 0; j < 8; ++j)
-                    v = fmaf(bf2f(a[j]), bf2f(b[j]), v);
+                    v = fmaf(bf2f(av[j]), bf2f(bv[j]), v);
             }
         }
-        if (bias != nullptr) v += bf2f(bias[col]);
-        if (act == ACT_GELU) v = gelu_f(v);
-        else if (act == ACT_TANH) v = tanhf(v);
-        if (residual != nullptr) v += bf2f(residual[(long)row * N + col]);
-        out[(long)row * N + col] = f2bf(v);
+        if (a.bias != nullptr) v += bf2f(a.bias[col]);
+        if (a.act == ACT_GELU) v = gelu_f(v);
+        else if (a.act == ACT_TANH) v = tanhf(v);
+        if (a.residual != nullptr) v += bf2f(a.residual[(long)row * N + col]);
+        a.out[(long)row * N + col] = f2bf(v);
     }
+}
+
+// Activation, residual and rounding of up to 8 adjacent columns.
+__device__ __forceinline__ void finish8(float (&v)[8], const __bf16* residual,
+                                        __bf16* out, long at, int count,
+                                        bool whole, int act) {
+    if (act == ACT_GELU) {
+        #pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = gelu_f(v[j]);
+    } else if (act == ACT_TANH) {
+        #pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = tanhf(v[j]);
+    }
+    if (residual != nullptr) {
+        const bf16x8 r = inner_load(residual + at, 0, count, whole);
+        #pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] += bf2f(r[j]);
+    }
+    bf16x8 o;
+    #pragma unroll
+    for (int j = 0; j < 8; ++j) o[j] = f2bf(v[j]);
+    if (whole) {
+        *reinterpret_cast<bf16x8*>(out + at) = o;
+    } else {
+        #pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j < count) out[at + j] = o[j];
+    }
+}
+
+// The whole projection of many rows, as y^T = W x^T on 32x32x16 MFMAs: a lane
+// then holds columns of one row, so the row's adapter is a property of the
+// lane, and four adjacent columns leave together. A block computes BN columns
+// of BM rows in WN x WM waves of 32 NI columns by 32 MI rows each. Slices of
+// 64 of K go to LDS by LDS-DMA, two buffers; operands are read from LDS one
+// step of 16 ahead of their MFMAs, also across slices: the barrier that ends
+// a slice comes before its last step, whose operands are in registers by
+// then.
+
+// Columns and rows of the block: in each XCD's contiguous share of the work,
+// bands of 8 row blocks, column by column, so that the blocks that run at the
+// same time share slices of both operands in that XCD's L2.
+__device__ __forceinline__ void product_place(const ProductArgs& a, int& bm,
+                                              int& bn) {
+    const int id = xcd_contiguous(blockIdx.x, gridDim.x);
+    const int band = id / (8 * a.n_blocks), first = band * 8;
+    const int high = min(8, a.m_blocks - first);
+    const int in = id - band * 8 * a.n_blocks;
+    bm = first + in % high;
+    bn = in / high;
+}
+
+template <int NI, int MI, int WN, int WM, int BK, int BUFS>
+__global__ __launch_bounds__(64 * WN * WM, 2) void adapter_product_kernel(
+        ProductArgs a) {
+    constexpr int BN = 32 * NI * WN, BM = 32 * MI * WM, THREADS = 64 * WN * WM;
+    constexpr int CH = BK / 8, STEPS = BK / 16;
+    constexpr int SLICE = (BN + BM) * BK;       // one buffer: [W | x] images
+    constexpr int PR = 64 / CH;                 // rows a piece of 1 KiB
+    constexpr int PIECES = (BN + BM) / PR / (WN * WM);
+    typedef TileVec<__bf16>::v8 v8;
+    __shared__ __attribute__((aligned(256))) __bf16 smem[BUFS * SLICE];
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int l31 = lane & 31, hi = lane >> 5;
+    const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wn = wid % WN, wm = wid / WN;
+    int bm, bn;
+    product_place(a, bm, bn);
+    const int n0 = bn * BN, m0 = bm * BM;
+
+    // The adapters among the block's rows, found one after another by all
+    // waves alike: lane l holds those of rows l, l + 64, .. not yet found.
+    int left[(BM + 63) / 64];
+    #pragma unroll
+    for (int i = 0; i < (BM + 63) / 64; ++i) {
+        const int r = i * 64 + lane, row = m0 + r;
+        const int v = r < BM && row < a.M
+            ? a.ad.row_ids[row / a.ad.rows_per_id] : -1;
+        left[i] = v < a.ad.n_adapters ? v : -1;
+    }
+    const auto next_adapter = [&] {
+        int found = -1;
+        #pragma unroll
+        for (int i = 0; i < (BM + 63) / 64; ++i) {
+            const unsigned long long has = __ballot(left[i] >= 0);
+            if (found < 0 && has)
+                found = __builtin_amdgcn_readlane(left[i],
+                                                  __builtin_ctzll(has));
+        }
+        #pragma unroll
+        for (int i = 0; i < (BM + 63) / 64; ++i)
+            if (left[i] == found) left[i] = -1;
+        return found;
+    };
+    // this lane's rows
+    int id[MI];
+    #pragma unroll
+    for (int m = 0; m < MI; ++m) {
+        const int row = m0 + (wm * MI + m) * 32 + l31;
+        id[m] = row < a.M ? a.ad.row_ids[row / a.ad.rows_per_id] : -1;
+    }
+    int adapter = next_adapter();
+
+    // this wave's pieces of a slice; rows behind the last repeat it and are
+    // not stored
+    const __bf16* src[PIECES];
+    #pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+        const int r = (wid * PIECES + i) * PR + lane / CH;
+        const int c = (lane % CH) ^ tile_key<CH>(r);
+        src[i] = (r < BN ? a.w + (long)min(n0 + r, a.N - 1) * a.K
+                         : a.x + (long)min(m0 + r - BN, a.M - 1) * a.K)
+                 + c * 8;
+    }
+    const int slices = (a.K + BK - 1) / BK;
+    // the first adapter's product is staged as one slice more
+    const int staged = slices + (adapter >= 0 ? 1 : 0);
+    // [up | inner] from column k of the rank; columns behind the rank repeat
+    // the last ones and are not used
+    const auto stage_adapter = [&](int which, int k, int buf) {
+        __bf16* image = smem + buf * SLICE;
+        const __bf16* up = a.ad.up + (long)which * a.N * a.ad.rank;
+        #pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const int r = (wid * PIECES + i) * PR + lane / CH;
+            const int c = k + ((lane % CH) ^ tile_key<CH>(r)) * 8;
+            const __bf16* from = r < BN
+                ? up + (long)min(n0 + r, a.N - 1) * a.ad.rank
+                    + min(c, a.ad.rank - 8)
+                : a.ad.inner + (long)min(m0 + r - BN, a.M - 1)
+                    * a.ad.rank_pad + min(c, a.ad.rank_pad - 8);
+            tile_load(from, image + (wid * PIECES + i) * 512);
+        }
+    };
+    const auto fast = [&](int t) {
+        return t == slices || (a.vec && (t + 1) * BK <= a.K);
+    };
+    const auto stage = [&](int t, int buf) {
+        __bf16* image = smem + buf * SLICE;
+        if (t == slices) {
+            stage_adapter(adapter, 0, buf);
+        } else if (fast(t)) {
+            #pragma unroll
+            for (int i = 0; i < PIECES; ++i)
+                tile_load(src[i] + t * BK,
+                          image + (wid * PIECES + i) * 512);
+        } else {
+            // the last part of a slice, or rows without alignment
+            #pragma unroll 1
+            for (int i = 0; i < PIECES; ++i) {
+                const int r = (wid * PIECES + i) * PR + lane / CH;
+                const int c = (lane % CH) ^ tile_key<CH>(r);
+                const __bf16* row = r < BN
+                    ? a.w + (long)min(n0 + r, a.N - 1) * a.K
+                    : a.x + (long)min(m0 + r - BN, a.M - 1) * a.K;
+                *reinterpret_cast<bf16x8*>(
+                    image + (wid * PIECES + i) * 512 + lane * 8) =
+                    inner_load(row, t * BK + c * 8, a.K, a.vec);
+            }
+        }
+    };
+
+    f32x16 acc[NI][MI] = {};
+    v8 fw[2][NI], fx[2][MI];
+    const unsigned lds = tile_lds(smem);
+    const unsigned base = tile_row_base<CH, 32>(lds, lane);
+    const auto read = [&](int buf, int step, int to) {
+        const unsigned at = base + buf * SLICE * 2;
+        #pragma unroll
+        for (int n = 0; n < NI; ++n)
+            fw[to][n] = tile_row_read<__bf16, CH, 32>(
+                at + wn * NI * 32 * BK * 2, n * 32, step);
+        #pragma unroll
+        for (int m = 0; m < MI; ++m)
+            fx[to][m] = tile_row_read<__bf16, CH, 32>(
+                at + (BN + wm * MI * 32) * BK * 2, m * 32, step);
+    };
+    const auto multiply = [&](int from) {
+        #pragma unroll
+        for (int n = 0; n < NI; ++n)
+            #pragma unroll
+            for (int m = 0; m < MI; ++m)
+                acc[n][m] = tile_mfma(fw[from][n], fx[from][m], acc[n][m]);
+    };
+    // Slice t has arrived for this wave, and its reads of the slice before
+    // are done; behind the barrier that holds for all waves. LDS-DMA arrives
+    // in order, so the pieces of later slices may stay on their way.
+    const auto arrive = [&](int t) {
+        if (BUFS == 3 && t + 1 < staged && fast(t + 1))
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"(PIECES)
+                         : "memory");
+        else
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+
+    #pragma unroll
+    for (int t = 0; t < BUFS - 1; ++t)
+        if (t < staged) stage(t, t);
+    arrive(0);
+    if (BUFS - 1 < staged) stage(BUFS - 1, BUFS - 1);
+    read(0, 0, 0);
+    int buf = 0;
+    for (int t = 0; t < slices; ++t) {
+        const int next = buf + 1 == BUFS ? 0 : buf + 1;
+        #pragma unroll
+        for (int step = 0; step < STEPS; ++step) {
+            if (step + 1 < STEPS) {
+                read(buf, step + 1, (step + 1) & 1);
+            } else if (t + 1 < slices) {
+                // all operands of slice t are in registers, so its buffer
+                // is free once every wave is here
+                arrive(t + 1);
+                if (t + BUFS < staged) stage(t + BUFS, buf);
+                read(next, 0, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(step & 1);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        buf = next;
+    }
+
+    // ---- the adapters of the block's rows: slices of [up | inner], the next
+    // one on its way while one is used
+    for (int k = 0; adapter >= 0;) {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        const int cur = adapter, k0 = k;
+        k += BK;
+        if (k >= a.ad.rank) {
+            adapter = next_adapter();
+            k = 0;
+        }
+        const int next = buf + 1 == BUFS ? 0 : buf + 1;
+        if (adapter >= 0) stage_adapter(adapter, k, next);
+        #pragma unroll
+        for (int step = 0; step < STEPS; ++step) {
+            if (k0 + step * 16 >= a.ad.rank) break;
+            read(buf, step, 0);
+            if (k0 + step * 16 + hi * 8 >= a.ad.rank)
+                #pragma unroll
+                for (int n = 0; n < NI; ++n) fw[0][n] = v8{};
+            #pragma unroll
+            for (int m = 0; m < MI; ++m) {
+                if (!__any(id[m] == cur)) continue;
+                if (__all(id[m] == cur)) {
+                    #pragma unroll
+                    for (int n = 0; n < NI; ++n)
+                        acc[n][m] = tile_mfma(fw[0][n], fx[0][m], acc[n][m]);
+                    continue;
+                }
+                // other requests' rows take nothing, not even the NaN of
+                // their own values times this adapter's
+                #pragma unroll
+                for (int n = 0; n < NI; ++n) {
+                    const f32x16 part =
+                        tile_mfma(fw[0][n], fx[0][m], f32x16{});
+                    #pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        acc[n][m][i] += id[m] == cur ? part[i] : 0.0f;
+                }
+            }
+        }
+        buf = next;
+    }
+
+    // ---- bias, activation, residual. The sums change hands through LDS, in
+    // as many passes as they need, so that a thread finishes 8 adjacent
+    // columns of a row and all accesses to memory are 16 B a lane. Chunk c (4
+    // columns) of row r lies at c ^ r: no conflict on either side.
+    constexpr int LDS = BUFS * SLICE * 2;
+    constexpr int LEAST = (BN * BM * 4 + LDS - 1) / LDS;
+    constexpr int PASSES = LEAST == 3 ? 4 : LEAST;
+    constexpr int MP = MI / PASSES, ROWS = 32 * MP * WM;
+    static_assert(MI % PASSES == 0, "whole tiles a pass");
+    constexpr int C4 = BN / 4, C8 = BN / 8;
+    static_assert(THREADS % C8 == 0, "a thread keeps its columns");
+    float* sums = reinterpret_cast<float*>(smem);
+    const int c8 = tid % C8, col = n0 + c8 * 8;
+    const bool whole = a.N % 8 == 0;
+    const int count = whole ? 8 : min(8, a.N - col);
+    float bias[8] = {};
+    if (a.bias != nullptr && col < a.N) {
+        const bf16x8 v = inner_load(a.bias + col, 0, count, whole);
+        #pragma unroll
+        for (int j = 0; j < 8; ++j) bias[j] = bf2f(v[j]);
+    }
+    #pragma unroll
+    for (int pass = 0; pass < PASSES; ++pass) {
+        __syncthreads();
+        #pragma unroll
+        for (int m = 0; m < MP; ++m) {
+            const int r = (wm * MP + m) * 32 + l31;
+            #pragma unroll
+            for (int n = 0; n < NI; ++n)
+                #pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const int c = (wn * NI + n) * 8 + g * 2 + hi;
+                    const f32x16& v = acc[n][pass * MP + m];
+                    *reinterpret_cast<f32x4*>(
+                        sums + r * BN + (c ^ (r % 16)) * 4) =
+                        f32x4{v[g * 4], v[g * 4 + 1], v[g * 4 + 2],
+                              v[g * 4 + 3]};
+                }
+        }
+        __syncthreads();
+        #pragma unroll 2
+        for (int r = tid / C8; r < ROWS; r += THREADS / C8) {
+            const int row = m0 + r / (32 * MP) * 32 * MI + pass * 32 * MP
+                            + r % (32 * MP);
+            if (row >= a.M || col >= a.N) continue;
+            float v[8];
+            #pragma unroll
+            for (int q = 0; q < 2; ++q)
+                *reinterpret_cast<f32x4*>(v + 4 * q) =
+                    *reinterpret_cast<const f32x4*>(
+                        sums + r * BN + ((2 * c8 + q) ^ (r % 16)) * 4);
+            #pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] += bias[j];
+            finish8(v, a.residual, a.out, (long)row * a.N + col, count,
+                    whole, a.act);
+        }
+    }
+}
+
+template <int NI, int MI, int WN, int WM, int BK, int BUFS>
+void product_launch(ProductArgs& a) {
+    a.n_blocks = (a.N + 32 * NI * WN - 1) / (32 * NI * WN);
+    a.m_blocks = (a.M + 32 * MI * WM - 1) / (32 * MI * WM);
+    hipLaunchKernelGGL((adapter_product_kernel<NI, MI, WN, WM, BK, BUFS>),
+                       dim3(a.n_blocks * a.m_blocks), dim3(64 * WN * WM), 0,
+                       pe_current_stream(), a);
+}
+
+void adapter_product(ProductArgs& a) {
+    static const int force = [] {
+        const char* s = std::getenv("PIPEEDGE_ADAPTER_T");
+        return s ? std::atoi(s) : 0;
+    }();
+    if (force == 1) product_launch<2, 4, 4, 2, 64, 2>(a);
+    else if (force == 2) product_launch<2, 2, 2, 2, 64, 2>(a);
+    else if (force == 3) product_launch<1, 1, 2, 2, 64, 2>(a);
+    else if (force == 4) product_launch<2, 4, 2, 2, 32, 3>(a);
+    else if (force == 5) product_launch<4, 2, 2, 2, 32, 3>(a);
+    else if (force == 6) product_launch<2, 2, 2, 2, 32, 3>(a);
+    else if (force == 7) product_launch<1, 1, 2, 2, 64, 3>(a);
+    else product_launch<2, 4, 2, 2, 32, 3>(a);
 }
 
 // Rows that the kernels for few rows take.
@@ -242,27 +613,22 @@ void adapter_inner(const InnerArgs& a) {
         return;
     }
     // columns a block: all of them up to 64, then 64 at a time
-    const int rows = (a.M + 15) / 16;
-    if (a.rank_pad <= 32)
-        hipLaunchKernelGGL((adapter_inner_kernel<2>), dim3(rows, 1), block, 0,
+    const dim3 grid((a.M + 15) / 16, (a.rank + 63) / 64);
+    if (a.rank <= 16)
+        hipLaunchKernelGGL((adapter_inner_kernel<1>), grid, block, 0,
+                           pe_current_stream(), a);
+    else if (a.rank <= 32)
+        hipLaunchKernelGGL((adapter_inner_kernel<2>), grid, block, 0,
                            pe_current_stream(), a);
     else
-        hipLaunchKernelGGL((adapter_inner_kernel<4>),
-                           dim3(rows, (a.rank_pad + 63) / 64), block, 0,
+        hipLaunchKernelGGL((adapter_inner_kernel<4>), grid, block, 0,
                            pe_current_stream(), a);
 }
 
 template <int NM>
-void adapter_step(const torch::Tensor& x, const torch::Tensor& w,
-                  const __bf16* bias, const __bf16* residual,
-                  torch::Tensor& out, const AdapterRows& rows, int act) {
-    const int M = x.size(0), N = w.size(0), K = x.size(1);
-    hipLaunchKernelGGL((adapter_step_kernel<NM>), dim3((N + 15) / 16),
-                       dim3(64 * STEP_WAVES), 0, pe_current_stream(),
-                       reinterpret_cast<const __bf16*>(x.data_ptr()),
-                       reinterpret_cast<const __bf16*>(w.data_ptr()), bias,
-                       residual, reinterpret_cast<__bf16*>(out.data_ptr()),
-                       rows, M, N, K, act, K % 8 == 0);
+void adapter_step(const ProductArgs& a) {
+    hipLaunchKernelGGL((adapter_step_kernel<NM>), dim3((a.N + 15) / 16),
+                       dim3(64 * STEP_WAVES), 0, pe_current_stream(), a);
 }
 
 torch::Tensor adapter_dense(const torch::Tensor& x) {
@@ -352,52 +718,57 @@ torch::Tensor adapter_linear_op(
 
     const auto x2d = adapter_dense(x.reshape({M, K}));
     const auto w = adapter_dense(weight);
-    c10::optional<torch::Tensor> res2d;
-    if (residual.has_value()) res2d = residual->reshape({M, N});
-    if (n == 0 || r == 0)
-        return std::get<0>(gemm_bf16(x2d, w, bias, act, res2d, 0,
-                                     c10::nullopt, c10::nullopt, c10::nullopt,
-                                     1e-12, false, nullptr))
-            .reshape(out_sizes);
-    const auto down_c = adapter_dense(down), up_c = adapter_dense(up);
+    const auto down_c = adapter_dense(down);
+    // the products of many rows read up 8 of the rank at a time
+    const bool pad_up = M > STEP_ROWS && r % 8 != 0;
+    const auto up_c = pad_up ? at::constant_pad_nd(up, {0, 8 - r % 8})
+                             : adapter_dense(up);
     const auto ids_c = ids.contiguous();
+    const auto tensor_or_none = [](c10::optional<torch::Tensor>& t) {
+        if (!t.has_value()) return (const __bf16*)nullptr;
+        t = adapter_dense(*t);
+        return reinterpret_cast<const __bf16*>(t->data_ptr());
+    };
     const int rank_pad = (r + 31) / 32 * 32;
-    auto inner = torch::empty({M, rank_pad}, x.options());
-    InnerArgs in = {};
-    in.x = reinterpret_cast<const __bf16*>(x2d.data_ptr());
-    in.down = reinterpret_cast<const __bf16*>(down_c.data_ptr());
-    in.row_ids = ids_c.data_ptr<int>();
-    torch::Tensor scales_c;
-    if (scales.has_value()) {
-        scales_c = scales->contiguous();
-        in.scales = scales_c.data_ptr<float>();
-    }
-    in.inner = reinterpret_cast<__bf16*>(inner.data_ptr());
-    in.M = M, in.K = K, in.n_adapters = n, in.rank = r;
-    in.rows_per_id = by_row ? 1 : M / x.size(0);
-    in.rank_pad = rank_pad;
-    in.vec = K % 8 == 0;
-    adapter_inner(in);
-    HIP_CHECK_LAST();
-    const AdapterRows rows = {inner.data_ptr(), up_c.data_ptr(),
-                              ids_c.data_ptr<int>(), in.rows_per_id, (int)n,
-                              (int)r, rank_pad};
-    if (M <= STEP_ROWS) {
-        auto out = torch::empty(out_sizes, x.options());
-        const auto pointer = [](c10::optional<torch::Tensor>& t) {
-            if (!t.has_value()) return (const __bf16*)nullptr;
-            t = t->contiguous();
-            return reinterpret_cast<const __bf16*>(t->data_ptr());
-        };
-        const auto* b = pointer(bias);
-        const auto* res = pointer(res2d);
-        if (M <= 16) adapter_step<1>(x2d, w, b, res, out, rows, act);
-        else if (M <= 32) adapter_step<2>(x2d, w, b, res, out, rows, act);
-        else adapter_step<4>(x2d, w, b, res, out, rows, act);
+    const bool any = n > 0 && r > 0;
+    auto inner = torch::empty({any ? M : 0, rank_pad}, x.options());
+    auto out = torch::empty(out_sizes, x.options());
+    ProductArgs a = {};
+    a.x = reinterpret_cast<const __bf16*>(x2d.data_ptr());
+    a.w = reinterpret_cast<const __bf16*>(w.data_ptr());
+    a.bias = tensor_or_none(bias);
+    a.residual = tensor_or_none(residual);
+    a.out = reinterpret_cast<__bf16*>(out.data_ptr());
+    a.M = M, a.N = N, a.K = K, a.act = act;
+    a.vec = K % 8 == 0;
+    a.ad.inner = reinterpret_cast<const __bf16*>(inner.data_ptr());
+    a.ad.up = reinterpret_cast<const __bf16*>(up_c.data_ptr());
+    a.ad.row_ids = ids_c.data_ptr<int>();
+    a.ad.rows_per_id = by_row ? 1 : M / x.size(0);
+    a.ad.n_adapters = any ? n : 0;      // without any, no id is inside
+    a.ad.rank = up_c.size(2), a.ad.rank_pad = rank_pad;
+    if (any) {
+        InnerArgs in = {};
+        in.x = a.x;
+        in.down = reinterpret_cast<const __bf16*>(down_c.data_ptr());
+        in.row_ids = a.ad.row_ids;
+        torch::Tensor scales_c;
+        if (scales.has_value()) {
+            scales_c = scales->contiguous();
+            in.scales = scales_c.data_ptr<float>();
+        }
+        in.inner = reinterpret_cast<__bf16*>(inner.data_ptr());
+        in.M = M, in.K = K, in.n_adapters = n, in.rank = r;
+        in.rows_per_id = a.ad.rows_per_id;
+        in.rank_pad = rank_pad;
+        in.vec = a.vec;
+        adapter_inner(in);
         HIP_CHECK_LAST();
-        return out;
     }
-    return std::get<0>(gemm_bf16(x2d, w, bias, act, res2d, 0, c10::nullopt,
-                                 c10::nullopt, c10::nullopt, 1e-12, false,
-                                 &rows)).reshape(out_sizes);
+    if (M <= 16) adapter_step<1>(a);
+    else if (M <= 32) adapter_step<2>(a);
+    else if (M <= STEP_ROWS) adapter_step<4>(a);
+    else adapter_product(a);
+    HIP_CHECK_LAST();
+    return out;
 }

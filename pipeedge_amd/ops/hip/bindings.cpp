@@ -4,8 +4,6 @@
 // every GPU tensor; there is no eager fallback on GPU (fail-loud contract).
 #include <torch/extension.h>
 
-#include "adapter.h"
-
 std::tuple<torch::Tensor, torch::Tensor> gemm_bf16(
         torch::Tensor a2d, torch::Tensor b,
         c10::optional<torch::Tensor> bias, int64_t act,
@@ -13,8 +11,7 @@ std::tuple<torch::Tensor, torch::Tensor> gemm_bf16(
         c10::optional<torch::Tensor> ln_stats = c10::nullopt,
         c10::optional<torch::Tensor> ln_s = c10::nullopt,
         c10::optional<torch::Tensor> ln_c = c10::nullopt,
-        double ln_eps = 1e-12, bool want_stats = false,
-        const AdapterRows* adapters = nullptr);
+        double ln_eps = 1e-12, bool want_stats = false);
 torch::Tensor ln_stats_bf16(torch::Tensor x);
 torch::Tensor debug_mfma_tile(torch::Tensor a, torch::Tensor b);
 torch::Tensor layernorm_bf16(torch::Tensor x, torch::Tensor weight,

@@ -19,7 +19,6 @@
 
 #include <cstdlib>
 
-#include "adapter.h"
 #include "common.h"
 
 namespace {
@@ -81,93 +80,7 @@ struct EpilogueArgs {
     // stats_out[parts][M][2]; plain stores, no zeroing needed
     float* stats_out;        // or nullptr
     int stats_parts;
-    // low-rank adapters: row m belongs to adapter row_ids[m / rows_per_id]
-    // (none if outside 0 .. n_adapters-1) and adds
-    // inner[m] . up[id][col] before bias and activation
-    const __bf16* inner;     // [M][rank_pad], zero behind rank, or nullptr
-    const __bf16* up;        // [n_adapters][N][rank]
-    const int* row_ids;
-    int rows_per_id, n_adapters, rank, rank_pad;
 };
-
-// Adds the adapters' part to a wave's accumulators: for each adapter that
-// occurs among its rows, the products run over the rank and the other rows
-// drop them. Rows of one request lie together, so
-// most waves find one adapter; a wave of 64 requests' single rows reads each
-// of their matrices once, which no order of work could save.
-template <int MI, int NI>
-__device__ __forceinline__ void adapter_accumulate(
-        f32x4 (&acc)[MI][NI], const EpilogueArgs& ep, int row0, int col0,
-        int lane) {
-    const int l15 = lane & 15, k0 = (lane >> 4) * 8;
-    int id[MI];
-    #pragma unroll
-    for (int mi = 0; mi < MI; ++mi) {
-        const int row = row0 + mi * 16 + l15;
-        int v = row < ep.M ? ep.row_ids[row / ep.rows_per_id] : -1;
-        id[mi] = v < ep.n_adapters ? v : -1;
-    }
-    while (true) {
-        int cur = -1;
-        #pragma unroll
-        for (int mi = 0; mi < MI; ++mi) {
-            const unsigned long long has = __ballot(id[mi] >= 0);
-            if (cur < 0 && has)
-                cur = __builtin_amdgcn_readlane(id[mi],
-                                                __builtin_ctzll(has));
-        }
-        if (cur < 0) break;
-        const __bf16* up = ep.up + (long)cur * ep.N * ep.rank;
-        for (int k = k0; k < ep.rank_pad + k0; k += 32) {
-            bf16x8 b[NI];
-            #pragma unroll
-            for (int ni = 0; ni < NI; ++ni) {
-                const int col = min(col0 + ni * 16 + l15, ep.N - 1);
-                const __bf16* p = up + (long)col * ep.rank + k;
-                b[ni] = bf16x8{};
-                if (ep.rank % 8 == 0) {
-                    if (k < ep.rank)
-                        b[ni] = *reinterpret_cast<const bf16x8*>(p);
-                } else {
-                    #pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        if (k + j < ep.rank) b[ni][j] = p[j];
-                }
-            }
-            #pragma unroll
-            for (int mi = 0; mi < MI; ++mi) {
-                const unsigned mine = (unsigned)__ballot(id[mi] == cur)
-                                      & 0xffffu;
-                if (mine == 0) continue;
-                bf16x8 a = {};
-                if (id[mi] == cur)
-                    a = *reinterpret_cast<const bf16x8*>(
-                        ep.inner + (long)(row0 + mi * 16 + l15) * ep.rank_pad
-                        + k);
-                if (mine == 0xffffu) {
-                    #pragma unroll
-                    for (int ni = 0; ni < NI; ++ni)
-                        acc[mi][ni] =
-                            mfma_16x16x32_bf16(a, b[ni], acc[mi][ni]);
-                    continue;
-                }
-                // other requests' rows take nothing, not even the NaN of
-                // zero times an infinite weight
-                const unsigned rows = mine >> ((lane >> 4) * 4);
-                #pragma unroll
-                for (int ni = 0; ni < NI; ++ni) {
-                    const f32x4 part = mfma_16x16x32_bf16(a, b[ni], f32x4{});
-                    #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        acc[mi][ni][r] += (rows >> r) & 1 ? part[r] : 0.0f;
-                }
-            }
-        }
-        #pragma unroll
-        for (int mi = 0; mi < MI; ++mi)
-            if (id[mi] == cur) id[mi] = -1;
-    }
-}
 
 // cooperative per-block LN-coefficient pass: thread t < TBM sums row
 // (bm + t)'s partials and writes (mu, rstd) into the (reused) LDS tile -
@@ -196,8 +109,7 @@ __device__ __forceinline__ void ln_coeffs_to_lds(
     __syncthreads();
 }
 
-// EPM: 0 plain, 1 ln-in, 2 stats-out, 3 adapters (added to acc before)
-template <int MI, int NI, int EPM>
+template <int MI, int NI, int EPM>  // EPM: 0 plain, 1 ln-in, 2 stats-out
 __device__ __forceinline__ void gemm_epilogue(
         const f32x4 (&acc)[MI][NI], const EpilogueArgs& ep, int bm, int bn,
         int wm, int wn, int lane, int part_idx, const float* lnbuf) {
@@ -369,8 +281,6 @@ __global__ __launch_bounds__(256) void gemm_bf16_glds_kernel(
     float* lnbuf = reinterpret_cast<float*>(&smem[0][0][0]);
     if constexpr (EPM == 1)
         ln_coeffs_to_lds<TBM>(ep, bm, tid, lnbuf);
-    if constexpr (EPM == 3)
-        adapter_accumulate<MI, NI>(acc, ep, bm + wm, bn + wn, lane);
     gemm_epilogue<MI, NI, EPM>(acc, ep, bm, bn, wm, wn, lane,
                                (bn / TBN) * 2 + (wid & 1), lnbuf);
 }
@@ -508,8 +418,6 @@ __global__ __launch_bounds__(256) void gemm_bf16_glds3_kernel(
     float* lnbuf = reinterpret_cast<float*>(&smem[0][0][0]);
     if constexpr (EPM == 1)
         ln_coeffs_to_lds<TBM>(ep, bm, tid, lnbuf);
-    if constexpr (EPM == 3)
-        adapter_accumulate<MI, NI>(acc, ep, bm + wm, bn + wn, lane);
     gemm_epilogue<MI, NI, EPM>(acc, ep, bm, bn, wm, wn, lane,
                                (bn / TBN) * 2 + (wid & 1), lnbuf);
 }
@@ -705,7 +613,7 @@ __global__ __launch_bounds__(256) void gemm_bf16_splitk_kernel(
 //   <4,4,3>: 128x256 tile, 144 KiB LDS, 1 block/CU
 //   <8,4,2>: 256x256 tile, 128 KiB LDS, 1 block/CU (classic 2-buffer)
 // ---------------------------------------------------------------------------
-template <int MI, int NI, int NBUF, bool XCD = true, int EPM = 0>
+template <int MI, int NI, int NBUF, bool XCD = true>
 __global__ __launch_bounds__(512) void gemm_bf16_glds8_kernel(
         const __bf16* __restrict__ A, const __bf16* __restrict__ B,
         __bf16* __restrict__ C, int M, int N, int K, EpilogueArgs ep) {
@@ -822,9 +730,7 @@ __global__ __launch_bounds__(512) void gemm_bf16_glds8_kernel(
         }
     }
     __builtin_amdgcn_s_barrier();
-    if constexpr (EPM == 3)
-        adapter_accumulate<MI, NI>(acc, ep, bm + wm, bn + wn, lane);
-    gemm_epilogue<MI, NI, EPM>(acc, ep, bm, bn, wm, wn, lane, 0, nullptr);
+    gemm_epilogue<MI, NI, 0>(acc, ep, bm, bn, wm, wn, lane, 0, nullptr);
 }
 
 // ---------------------------------------------------------------------------
@@ -1026,8 +932,6 @@ __global__ __launch_bounds__(256) void gemm_bf16_generic_kernel(
     float* lnbuf = reinterpret_cast<float*>(&As[0][0]);
     if constexpr (EPM == 1)
         ln_coeffs_to_lds<BM>(ep, bm, tid, lnbuf);
-    if constexpr (EPM == 3)
-        adapter_accumulate<2, 2>(acc, ep, bm + wm, bn + wn, lane);
     gemm_epilogue<2, 2, EPM>(acc, ep, bm, bn, wm, wn, lane,
                              (bn / BN) * 2 + (wid & 1), lnbuf);
 }
@@ -1040,8 +944,7 @@ std::tuple<torch::Tensor, torch::Tensor> gemm_bf16(
         c10::optional<torch::Tensor> residual2d, int64_t tile,
         c10::optional<torch::Tensor> ln_stats,
         c10::optional<torch::Tensor> ln_s,
-        c10::optional<torch::Tensor> ln_c, double ln_eps, bool want_stats,
-        const AdapterRows* adapters) {
+        c10::optional<torch::Tensor> ln_c, double ln_eps, bool want_stats) {
     TORCH_CHECK(a2d.is_cuda() && a2d.dtype() == torch::kBFloat16,
                 "gemm: A must be bf16 on GPU");
     TORCH_CHECK(b.dtype() == torch::kBFloat16, "gemm: B must be bf16");
@@ -1072,8 +975,7 @@ std::tuple<torch::Tensor, torch::Tensor> gemm_bf16(
 
     EpilogueArgs ep{bias_p, res_p, cp, M, N, (int)act,
                     nullptr, 0, nullptr, nullptr, (float)ln_eps, K,
-                    1.0f / K, nullptr, 0, nullptr, nullptr, nullptr, 0, 0, 0,
-                    0};
+                    1.0f / K, nullptr, 0};
     if (ln_stats.has_value()) {
         TORCH_CHECK(ln_s.has_value() && ln_c.has_value(),
                     "gemm: ln_stats requires ln_s and ln_c");
@@ -1085,17 +987,6 @@ std::tuple<torch::Tensor, torch::Tensor> gemm_bf16(
         ep.ln_parts = ln_stats->size(1);
         ep.ln_s = ln_s->data_ptr<float>();
         ep.ln_c = ln_c->data_ptr<float>();
-    }
-    if (adapters != nullptr) {
-        TORCH_CHECK(ep.ln_stats == nullptr && !want_stats,
-                    "gemm: adapters exclude the other epilogue modes");
-        ep.inner = reinterpret_cast<const __bf16*>(adapters->inner);
-        ep.up = reinterpret_cast<const __bf16*>(adapters->up);
-        ep.row_ids = adapters->row_ids;
-        ep.rows_per_id = adapters->rows_per_id;
-        ep.n_adapters = adapters->n_adapters;
-        ep.rank = adapters->rank;
-        ep.rank_pad = adapters->rank_pad;
     }
     int t = 0;
     if (K % BK == 0) {
@@ -1144,9 +1035,6 @@ std::tuple<torch::Tensor, torch::Tensor> gemm_bf16(
             else if (midt != 0 && M >= 256) t = midt;
             else t = 5;
         }
-        // the adapters' epilogue is built for the tiles chosen above
-        if (adapters != nullptr && t != 7 && t != 13 && t != 14 && t != 15)
-            t = 5;
         if (t == 4 && K % (2 * BK) != 0) t = 1;
         if (t == 6 && K % (2 * BK) != 0) t = 5;
 
@@ -1164,35 +1052,6 @@ std::tuple<torch::Tensor, torch::Tensor> gemm_bf16(
     }
     const int epm = ep.ln_stats != nullptr ? 1
                     : (ep.stats_out != nullptr ? 2 : 0);
-    if (adapters != nullptr) {
-        const dim3 grid64((M + BM - 1) / BM, (N + BN - 1) / BN);
-        const auto stream = pe_current_stream();
-        if (K % BK != 0)
-            hipLaunchKernelGGL((gemm_bf16_generic_kernel<3>), grid64,
-                               dim3(256), 0, stream, ap, bp, cp, M, N, K, ep);
-        else if (t == 13)
-            hipLaunchKernelGGL((gemm_bf16_glds8_kernel<8, 4, 2, true, 3>),
-                               dim3((M + 255) / 256, (N + 255) / 256),
-                               dim3(512), 0, stream, ap, bp, cp, M, N, K, ep);
-        else if (t == 14)
-            hipLaunchKernelGGL((gemm_bf16_glds8_kernel<8, 2, 3, true, 3>),
-                               dim3((M + 255) / 256, (N + 127) / 128),
-                               dim3(512), 0, stream, ap, bp, cp, M, N, K, ep);
-        else if (t == 15)
-            hipLaunchKernelGGL((gemm_bf16_glds8_kernel<8, 3, 2, true, 3>),
-                               dim3((M + 255) / 256, (N + 191) / 192),
-                               dim3(512), 0, stream, ap, bp, cp, M, N, K, ep);
-        else if (t == 7)
-            hipLaunchKernelGGL((gemm_bf16_glds3_kernel<2, 2, true, 3, 3>),
-                               grid64, dim3(256), 0, stream, ap, bp, cp, M, N,
-                               K, ep);
-        else
-            hipLaunchKernelGGL((gemm_bf16_glds_kernel<2, 2, 1, true, 3>),
-                               grid64, dim3(256), 0, stream, ap, bp, cp, M, N,
-                               K, ep);
-        HIP_CHECK_LAST();
-        return {out, stats};
-    }
 #define PE_LAUNCH_GLDS(MI_, NI_, KT_, XCD_, GRID_)                           \
     do {                                                                     \
         if (epm == 1)                                                        \

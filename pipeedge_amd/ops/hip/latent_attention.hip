@@ -15,7 +15,7 @@
 
 #include <c10/core/DeviceGuard.h>
 
-#include "latent_common.h"
+#include "mfma_tiles.h"
 
 namespace {
 
@@ -40,8 +40,8 @@ __global__ __launch_bounds__(256, 2) void latent_attention_kernel(
         LatentArgs a) {
     constexpr int CN = DN / 8, CR = DR / 8;
     constexpr int NT = DN / 32;                 // output tiles a wave
-    typedef typename LatentVec<T>::v8 v8;
-    typedef LatentSoftmax<T> softmax;
+    typedef typename TileVec<T>::v8 v8;
+    typedef RunningTop<T> softmax;
     // two buffers of [nope | rope | value] images
     constexpr int TILE = KEYS * (2 * DN + DR);
     __shared__ __attribute__((aligned(256))) T smem[2 * TILE];
@@ -95,17 +95,17 @@ __global__ __launch_bounds__(256, 2) void latent_attention_kernel(
         for (int i = 0; i < CN / 4; ++i) {
             const int p = wid + 4 * i;
             const int r = p * (64 / CN) + lane / CN;
-            const int c = (lane % CN) ^ latent_key<CN>(r);
+            const int c = (lane % CN) ^ tile_key<CN>(r);
             const T* src = kv + min(tok0 + r, len - 1) * a.kv_s + c * 8;
-            latent_lds_load(src, base + p * 512);
-            latent_lds_load(src + DN, base + KEYS * (DN + DR) + p * 512);
+            tile_load(src, base + p * 512);
+            tile_load(src + DN, base + KEYS * (DN + DR) + p * 512);
         }
         #pragma unroll
         for (int i = 0; i < CR / 4; ++i) {
             const int p = wid + 4 * i;
             const int r = p * (64 / CR) + lane / CR;
-            const int c = (lane % CR) ^ latent_key<CR>(r);
-            latent_lds_load(kr + min(tok0 + r, len - 1) * a.r_s + c * 8,
+            const int c = (lane % CR) ^ tile_key<CR>(r);
+            tile_load(kr + min(tok0 + r, len - 1) * a.r_s + c * 8,
                             base + KEYS * DN + p * 512);
         }
     };
@@ -113,18 +113,18 @@ __global__ __launch_bounds__(256, 2) void latent_attention_kernel(
     f32x16 acc[NT] = {};
     float top = -INFINITY, sub = 0.0f, total = 0.0f;
 
-    const unsigned lds = latent_lds(smem);
+    const unsigned lds = tile_lds(smem);
     if (tiles > 0) stage(0, 0);
     for (int t = 0; t < tiles; ++t) {
         const unsigned image = lds + (t & 1) * TILE * 2;
-        const unsigned nope = latent_row_base<CN, 32>(image, lane);
+        const unsigned nope = tile_row_base<CN, 32>(image, lane);
         const unsigned rope =
-            latent_row_base<CR, 32>(image + KEYS * DN * 2, lane);
-        const unsigned value = latent_column_base<CN, 32>(
+            tile_row_base<CR, 32>(image + KEYS * DN * 2, lane);
+        const unsigned value = tile_column_base<CN, 32>(
             image + KEYS * (DN + DR) * 2, lane);
         // this wave's part of tile t has arrived; behind the barrier all
         // parts have, and every wave is done with the other buffer
-        latent_arrive();
+        tile_arrive();
         if (t + 1 < tiles) stage(t + 1, (t + 1) & 1);
         const int tok0 = t * KEYS;
         if (tok0 > wave_last) continue;
@@ -134,13 +134,13 @@ __global__ __launch_bounds__(256, 2) void latent_attention_kernel(
         for (int i = 0; i < DN / 16; ++i)
             #pragma unroll
             for (int m = 0; m < 2; ++m)
-                s[m] = latent_mfma(latent_row_read<T, CN, 32>(nope, m * 32, i),
+                s[m] = tile_mfma(tile_row_read<T, CN, 32>(nope, m * 32, i),
                                    bq[i], s[m]);
         #pragma unroll
         for (int i = 0; i < DR / 16; ++i)
             #pragma unroll
             for (int m = 0; m < 2; ++m)
-                s[m] = latent_mfma(latent_row_read<T, CR, 32>(rope, m * 32, i),
+                s[m] = tile_mfma(tile_row_read<T, CR, 32>(rope, m * 32, i),
                                    bq[DN / 16 + i], s[m]);
 
         if (__any(limit < tok0 + KEYS - 1)) {
@@ -185,10 +185,10 @@ __global__ __launch_bounds__(256, 2) void latent_attention_kernel(
                 float p[8];
                 #pragma unroll
                 for (int j = 0; j < 8; ++j) p[j] = s[m][8 * c + j];
-                const v8 w = latent_weights<T>(p);
+                const v8 w = tile_weights<T>(p);
                 #pragma unroll
                 for (int n = 0; n < NT; ++n)
-                    acc[n] = latent_mfma(latent_column_read<T, CN, 32>(
+                    acc[n] = tile_mfma(tile_column_read<T, CN, 32>(
                         value, m * 32 + c * 16, n), w, acc[n]);
             }
     }
@@ -202,11 +202,11 @@ __global__ __launch_bounds__(256, 2) void latent_attention_kernel(
         for (int n = 0; n < NT; ++n)
             #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                typename LatentVec<T>::v4 o;
+                typename TileVec<T>::v4 o;
                 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                     o[j] = (T)(acc[n][g * 4 + j] * inv);
-                *reinterpret_cast<typename LatentVec<T>::v4*>(
+                *reinterpret_cast<typename TileVec<T>::v4*>(
                     out + n * 32 + g * 8) = o;
             }
     }

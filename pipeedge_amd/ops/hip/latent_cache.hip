@@ -28,7 +28,7 @@
 
 #include <c10/core/DeviceGuard.h>
 
-#include "latent_common.h"
+#include "mfma_tiles.h"
 
 namespace {
 
@@ -135,8 +135,8 @@ void latent_cache_kernel(CacheArgs a) {
     constexpr bool ALONE = WR == 1;
     constexpr int PIECES = GROUPS * CL / 8 + GROUPS * CR / 8;
     static_assert(!ALONE || (GROUPS == 4 && PIECES < 64), "counted waits");
-    typedef typename LatentVec<T>::v8 v8;
-    typedef LatentSoftmax<T> softmax;
+    typedef typename TileVec<T>::v8 v8;
+    typedef RunningTop<T> softmax;
     // WT shares of two buffers of [latent | rope] images
     __shared__ __attribute__((aligned(256))) T smem[WT * 2 * TILE];
 
@@ -145,7 +145,7 @@ void latent_cache_kernel(CacheArgs a) {
     const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int group = wid % WR, share = wid / WR;
     T* const images = smem + share * 2 * TILE;
-    const unsigned lds = latent_lds(images);
+    const unsigned lds = tile_lds(images);
 
     const long total = cache_total(a, lane);
     long at = run_start(total, blockIdx.x, gridDim.x);
@@ -198,12 +198,12 @@ void latent_cache_kernel(CacheArgs a) {
             // tokens, of the rotary part rows p * RR ..
             constexpr int PR = 64 / CL, RR = 64 / CR;
             const auto latent_chunk = [&](int r) {
-                return ((lane % CL) ^ latent_key<CL>(group * GROUPS * 8 + r))
+                return ((lane % CL) ^ tile_key<CL>(group * GROUPS * 8 + r))
                        * 16;
             };
             const auto rotary_chunk = [&](int r) {
                 return R * 2 + ((lane % CR)
-                    ^ latent_key<CR>(group * GROUPS * 8 + r)) * 16;
+                    ^ tile_key<CR>(group * GROUPS * 8 + r)) * 16;
             };
             if (a.page_of_groups) {
                 // groups of 8 tokens never straddle a page: their places
@@ -223,7 +223,7 @@ void latent_cache_kernel(CacheArgs a) {
                 for (int p = 0; p < GROUPS * 8 / PR; ++p) {
                     const int r = p * PR + (PR == 1 ? 0 : lane / CL);
                     const CacheGroup& f = from[p * PR / 8];
-                    latent_lds_load(
+                    tile_load(
                         f.at + min(r % 8, f.last) * step + latent_chunk(r),
                         image + p * PR * R);
                 }
@@ -234,7 +234,7 @@ void latent_cache_kernel(CacheArgs a) {
                     if (RR == 16 && GROUPS > 1 && lane >= 32)
                         f = from[(p * RR / 8 + 1) % GROUPS];
                     if (r < GROUPS * 8)
-                        latent_lds_load(
+                        tile_load(
                             f.at + min(r % 8, f.last) * step
                             + rotary_chunk(r), rotary + p * RR * DR);
                 }
@@ -248,7 +248,7 @@ void latent_cache_kernel(CacheArgs a) {
                 #pragma unroll
                 for (int p = 0; p < GROUPS * 8 / PR; ++p) {
                     const int r = p * PR + lane / CL;
-                    latent_lds_load(
+                    tile_load(
                         reinterpret_cast<const char*>(a.cache)
                         + __shfl(place, r) + latent_chunk(r),
                         image + p * PR * R);
@@ -258,7 +258,7 @@ void latent_cache_kernel(CacheArgs a) {
                     const int r = p * RR + lane / CR;
                     const long from = __shfl(place, r);
                     if (r < GROUPS * 8)
-                        latent_lds_load(
+                        tile_load(
                             reinterpret_cast<const char*>(a.cache) + from
                             + rotary_chunk(r), rotary + p * RR * DR);
                 }
@@ -280,14 +280,14 @@ void latent_cache_kernel(CacheArgs a) {
                 else
                     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             } else {
-                latent_arrive();
+                tile_arrive();
                 if (t + 1 < t1) stage(t + 1, (t + 1) & 1);
             }
             const unsigned image = lds + (t & 1) * TILE * 2;
-            const unsigned latent = latent_row_base<CL, 16>(image, lane);
-            const unsigned rope = latent_row_base<CR, 16>(
+            const unsigned latent = tile_row_base<CL, 16>(image, lane);
+            const unsigned rope = tile_row_base<CR, 16>(
                 image + TOKENS * R * 2, lane);
-            const unsigned value = latent_column_base<CL, 16>(image, lane);
+            const unsigned value = tile_column_base<CL, 16>(image, lane);
             const int tok0 = t * KEYS + share * TOKENS;
 
             if (live) {
@@ -296,13 +296,13 @@ void latent_cache_kernel(CacheArgs a) {
             for (int i = 0; i < R / 32; ++i)
                 #pragma unroll
                 for (int m = 0; m < SUB; ++m)
-                    s[m] = latent_mfma(latent_row_read<T, CL, 16>(
+                    s[m] = tile_mfma(tile_row_read<T, CL, 16>(
                         latent, m * 16, i), bq[i], s[m]);
             #pragma unroll
             for (int i = 0; i < DR / 32; ++i)
                 #pragma unroll
                 for (int m = 0; m < SUB; ++m)
-                    s[m] = latent_mfma(latent_row_read<T, CR, 16>(
+                    s[m] = tile_mfma(tile_row_read<T, CR, 16>(
                         rope, m * 16, i), bq[R / 32 + i], s[m]);
 
             if (__any(limit < tok0 + TOKENS - 1)) {
@@ -345,10 +345,10 @@ void latent_cache_kernel(CacheArgs a) {
                 float p[8];
                 #pragma unroll
                 for (int j = 0; j < 8; ++j) p[j] = s[m + j / 4][j % 4];
-                const v8 w = latent_weights<T>(p);
+                const v8 w = tile_weights<T>(p);
                 #pragma unroll
                 for (int n = 0; n < NT; ++n)
-                    acc[n] = latent_mfma(latent_column_read<T, CL, 16>(
+                    acc[n] = tile_mfma(tile_column_read<T, CL, 16>(
                         value, m * 16, n), w, acc[n]);
             }
             }
@@ -405,10 +405,10 @@ void latent_cache_kernel(CacheArgs a) {
                          + ((long)seq * a.rows + row) * R + quad * 4;
                 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    typename LatentVec<T>::v4 o;
+                    typename TileVec<T>::v4 o;
                     #pragma unroll
                     for (int j = 0; j < 4; ++j) o[j] = (T)(acc[n][j] * inv);
-                    *reinterpret_cast<typename LatentVec<T>::v4*>(
+                    *reinterpret_cast<typename TileVec<T>::v4*>(
                         out + n * 16) = o;
                 }
             } else {

@@ -1,40 +1,40 @@
-// Pieces shared by the two forms of latent attention: the swizzled LDS
-// images that LDS-DMA fills, their two kinds of fragment reads, and the
-// running reference of the softmax.
+// Pieces shared by the kernels built from swizzled LDS images: LDS-DMA into
+// them, the two kinds of fragment reads, and the running reference of a
+// softmax.
 #pragma once
 
 #include "common.h"
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-template <typename T> struct LatentVec;
-template <> struct LatentVec<__bf16> {
+template <typename T> struct TileVec;
+template <> struct TileVec<__bf16> {
     typedef __bf16 v8 __attribute__((ext_vector_type(8)));
     typedef __bf16 v4 __attribute__((ext_vector_type(4)));
 };
-template <> struct LatentVec<_Float16> {
+template <> struct TileVec<_Float16> {
     typedef _Float16 v8 __attribute__((ext_vector_type(8)));
     typedef _Float16 v4 __attribute__((ext_vector_type(4)));
 };
 
-__device__ __forceinline__ f32x16 latent_mfma(LatentVec<__bf16>::v8 a,
-                                              LatentVec<__bf16>::v8 b,
+__device__ __forceinline__ f32x16 tile_mfma(TileVec<__bf16>::v8 a,
+                                              TileVec<__bf16>::v8 b,
                                               f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
-__device__ __forceinline__ f32x16 latent_mfma(LatentVec<_Float16>::v8 a,
-                                              LatentVec<_Float16>::v8 b,
+__device__ __forceinline__ f32x16 tile_mfma(TileVec<_Float16>::v8 a,
+                                              TileVec<_Float16>::v8 b,
                                               f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
 
-__device__ __forceinline__ f32x4 latent_mfma(LatentVec<__bf16>::v8 a,
-                                             LatentVec<__bf16>::v8 b,
+__device__ __forceinline__ f32x4 tile_mfma(TileVec<__bf16>::v8 a,
+                                             TileVec<__bf16>::v8 b,
                                              f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
-__device__ __forceinline__ f32x4 latent_mfma(LatentVec<_Float16>::v8 a,
-                                             LatentVec<_Float16>::v8 b,
+__device__ __forceinline__ f32x4 tile_mfma(TileVec<_Float16>::v8 a,
+                                             TileVec<_Float16>::v8 b,
                                              f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
@@ -51,7 +51,7 @@ __device__ __forceinline__ f32x4 latent_mfma(LatentVec<_Float16>::v8 a,
 // Rows of 16k + 8 chunks alternate between two halves already, rows of
 // 8k + 4 between four quarters.
 template <int CH>
-__device__ __forceinline__ constexpr int latent_key(int row) {
+__device__ __forceinline__ constexpr int tile_key(int row) {
     if constexpr (CH % 16 == 0)
         return ((row & 3) << 2) | (((row >> 2) & 1) << 1) | ((row >> 3) & 1);
     else if constexpr (CH % 8 == 0)
@@ -61,7 +61,7 @@ __device__ __forceinline__ constexpr int latent_key(int row) {
 }
 
 // 16 bytes a lane from global memory into LDS at base + lane * 16
-__device__ __forceinline__ void latent_lds_load(const void* src, void* dst) {
+__device__ __forceinline__ void tile_load(const void* src, void* dst) {
     __builtin_amdgcn_global_load_lds(
         (const __attribute__((address_space(1))) unsigned int*)src,
         (__attribute__((address_space(3))) unsigned int*)dst, 16, 0, 0);
@@ -69,7 +69,7 @@ __device__ __forceinline__ void latent_lds_load(const void* src, void* dst) {
 
 // Wait for this wave's LDS-DMA, then for all waves. The clobbers keep LDS
 // accesses on their side of the barrier.
-__device__ __forceinline__ void latent_arrive() {
+__device__ __forceinline__ void tile_arrive() {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
@@ -77,7 +77,7 @@ __device__ __forceinline__ void latent_arrive() {
 
 // Chunks that a key permutes among each other.
 template <int CH>
-__device__ __forceinline__ constexpr int latent_group() {
+__device__ __forceinline__ constexpr int tile_group() {
     return CH % 16 == 0 ? 16 : CH % 8 == 0 ? 8 : 4;
 }
 
@@ -85,7 +85,7 @@ __device__ __forceinline__ constexpr int latent_group() {
 // at compile time only flips address bits inside a group of chunks or adds a
 // constant, since rows and images begin at multiples of a group.
 
-__device__ __forceinline__ unsigned latent_lds(const void* p) {
+__device__ __forceinline__ unsigned tile_lds(const void* p) {
     return (unsigned)reinterpret_cast<uintptr_t>(p);    // byte address
 }
 
@@ -95,28 +95,28 @@ __device__ __forceinline__ unsigned latent_lds(const void* p) {
 
 // Score operand: chunks (64 / M) i + l / M of row row0 + l % M
 template <int CH, int M>
-__device__ __forceinline__ unsigned latent_row_base(unsigned image,
+__device__ __forceinline__ unsigned tile_row_base(unsigned image,
                                                     int lane) {
     const int row = lane % M;
-    return image + row * CH * 16 + (((lane / M) ^ latent_key<CH>(row)) << 4);
+    return image + row * CH * 16 + (((lane / M) ^ tile_key<CH>(row)) << 4);
 }
 template <typename T, int CH, int M>
-__device__ __forceinline__ typename LatentVec<T>::v8 latent_row_read(
+__device__ __forceinline__ typename TileVec<T>::v8 tile_row_read(
         unsigned base, int row0, int i) {
-    constexpr int G = latent_group<CH>(), STEP = 64 / M;
+    constexpr int G = tile_group<CH>(), STEP = 64 / M;
     const unsigned at = (base ^ ((STEP * i % G) << 4))
                         + (STEP * i / G) * G * 16 + row0 * CH * 16;
     return *reinterpret_cast<const __attribute__((address_space(3)))
-        typename LatentVec<T>::v8*>((uintptr_t)at);
+        typename TileVec<T>::v8*>((uintptr_t)at);
 }
 
 template <typename T>
-__device__ __forceinline__ typename LatentVec<T>::v4 latent_tr_read(
+__device__ __forceinline__ typename TileVec<T>::v4 tile_tr_read(
         unsigned at) {
-    typedef __attribute__((address_space(3))) LatentVec<__bf16>::v4 lds_v4;
+    typedef __attribute__((address_space(3))) TileVec<__bf16>::v4 lds_v4;
     const auto r = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
         reinterpret_cast<lds_v4*>((uintptr_t)at));
-    return __builtin_bit_cast(typename LatentVec<T>::v4, r);
+    return __builtin_bit_cast(typename TileVec<T>::v4, r);
 }
 
 // Value operand, V^T[M columns from M n][tokens]: lane l gets column l % M.
@@ -126,34 +126,34 @@ __device__ __forceinline__ typename LatentVec<T>::v4 latent_tr_read(
 // read turns 4 rows of 16 columns, given as 4 adjacent elements by each of 16
 // lanes, into one column of 4 rows for each of them.
 template <int CH, int M>
-__device__ __forceinline__ unsigned latent_column_base(unsigned image,
+__device__ __forceinline__ unsigned tile_column_base(unsigned image,
                                                        int lane) {
     const int row = lane / M * 4 + ((lane & 15) >> 2);
     const int chunk = (lane % M >= 16 ? 2 : 0) + ((lane & 3) >> 1);
-    return image + row * CH * 16 + ((chunk ^ latent_key<CH>(row)) << 4)
+    return image + row * CH * 16 + ((chunk ^ tile_key<CH>(row)) << 4)
            + (lane & 1) * 8;
 }
 template <typename T, int CH, int M>
-__device__ __forceinline__ typename LatentVec<T>::v8 latent_column_read(
+__device__ __forceinline__ typename TileVec<T>::v8 tile_column_read(
         unsigned base, int row0, int n) {
-    constexpr int G = latent_group<CH>(), STEP = M / 8;
+    constexpr int G = tile_group<CH>(), STEP = M / 8;
     constexpr int NEXT = 256 / M;       // rows to the second read
     // 16 rows on, a row's key is the same; 8 rows on, one bit differs
     constexpr unsigned flip8 =
-        NEXT == 16 ? 0 : (latent_key<CH>(8) ^ latent_key<CH>(0)) << 4;
+        NEXT == 16 ? 0 : (tile_key<CH>(8) ^ tile_key<CH>(0)) << 4;
     const unsigned flip = (STEP * n % G) << 4;
     const unsigned add = (STEP * n / G) * G * 16 + row0 * CH * 16;
-    const auto lo = latent_tr_read<T>((base ^ flip) + add);
-    const auto hi = latent_tr_read<T>((base ^ flip ^ flip8) + add
+    const auto lo = tile_tr_read<T>((base ^ flip) + add);
+    const auto hi = tile_tr_read<T>((base ^ flip ^ flip8) + add
                                       + NEXT * CH * 16);
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
 // eight weights, rounded to the type of the values they multiply
 template <typename T>
-__device__ __forceinline__ typename LatentVec<T>::v8 latent_weights(
+__device__ __forceinline__ typename TileVec<T>::v8 tile_weights(
         const float (&w)[8]) {
-    typename LatentVec<T>::v8 r;
+    typename TileVec<T>::v8 r;
     #pragma unroll
     for (int j = 0; j < 8; ++j) r[j] = (T)w[j];
     return r;
@@ -165,10 +165,10 @@ __device__ __forceinline__ typename LatentVec<T>::v8 latent_weights(
 // weights then stay below 2^SLACK above their usual range, and sums are held
 // in 32 bits. fp16 weights end at 65504 and lose bits below 2^-14, so they
 // are shifted up by BIAS.
-template <typename T> struct LatentSoftmax {
+template <typename T> struct RunningTop {
     static constexpr float SLACK = 8.0f, BIAS = 0.0f;
 };
-template <> struct LatentSoftmax<_Float16> {
+template <> struct RunningTop<_Float16> {
     static constexpr float SLACK = 5.0f, BIAS = 8.0f;
 };
 

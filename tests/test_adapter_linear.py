@@ -109,8 +109,6 @@ def test_adapter_ids_outside(device):
     plain = ops.adapter_linear(x, w, down, up, none, bias)
     for i in (0, 2, 4, 5):
         assert torch.equal(out[i], plain[i])
-    if device == "cuda":
-        assert torch.equal(plain, ops.linear(x, w, bias))
     for empty in (down[:0], up[:0]), (down[:, :0], up[..., :0]):
         assert torch.equal(ops.adapter_linear(x, w, *empty, ids, bias), plain)
 
