@@ -388,7 +388,8 @@ def adapter_linear(x: Tensor, weight: Tensor, down: Tensor, up: Tensor,
     if bias is not None:
         y = y + bias.float()
     if act == "gelu":
-        y = torch.nn.functional.gelu(y)
+        # through erfc, which keeps its digits where 1 + erf cancels
+        y = y * (0.5 * torch.special.erfc(y * -math.sqrt(0.5)))
     elif act == "tanh":
         y = torch.tanh(y)
     elif act is not None:

@@ -55,7 +55,8 @@ def check(out, x, w, down, up, ids, bias=None, act=None, residual=None,
     bound = bound + y.abs() * half + 1e-30
     assert out.dtype == torch.bfloat16
     err = (out.double().cpu().reshape(y.shape) - y).abs()
-    assert (err <= bound).all(), (err / bound).max()
+    worst = (err / bound).max().item()
+    assert worst <= 1.0
 
 
 @pytest.mark.parametrize("device", DEVICES)
@@ -134,6 +135,30 @@ def test_adapter_isolation(device, shape):
             assert torch.equal(out[i, keep], want[i, keep])
         else:
             assert not torch.isfinite(out[i]).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("rows", [4, 96])
+def test_adapter_gelu_range(device, rows):
+    """The activation alone over its range: an identity projection, whose
+    sums are exact. Far out its value is exp(-x^2 / 2) times a slow factor;
+    an exponent of up to 2^7 that is rounded to 2^-24 of itself moves it by
+    2^-17, the rest by less than 2^-18. Then it is rounded once; results
+    below the smallest normal number may be anything below it."""
+    values = torch.cat((torch.linspace(-12, 12, 200),
+                        torch.tensor([0.0, -0.0, 1e-3, -1e-3, 30.0, -30.0,
+                                      3e38, -3e38])))
+    w = values.bfloat16().reshape(-1, 1).to(device)
+    x = torch.ones(rows, 1, device=device).bfloat16()
+    down = torch.zeros(1, 8, 1, device=device).bfloat16()
+    up = torch.zeros(1, w.shape[0], 8, device=device).bfloat16()
+    ids = torch.zeros(rows, dtype=torch.int32, device=device)
+    out = ops.adapter_linear(x, w, down, up, ids, act="gelu").double().cpu()
+    v = w.double().cpu().reshape(-1)
+    ref = v * 0.5 * torch.special.erfc(-v * 0.5 ** 0.5)
+    bound = ref.abs() * (2.0 ** -8 + 2.0 ** -16) + 2.0 ** -126
+    worst = ((out - ref).abs() / bound).max().item()
+    assert worst <= 1.0
 
 
 @pytest.mark.parametrize("device", DEVICES)

@@ -37,9 +37,8 @@ def check(out, ref, size, drift, dtype):
     out = out.double().cpu()
     bound = ref.abs() * half + size * (
         half + 2.0 * drift.unsqueeze(-1) + 2.0 ** -17) + 1e-7
-    assert torch.isfinite(out).all()
-    assert ((out - ref).abs() <= bound).all(), \
-        ((out - ref).abs() / bound).max()
+    worst = ((out - ref).abs() / bound).max().item()
+    assert worst <= 1.0             # also not if it is NaN
 
 
 def expanded_exact(q, kv, k_rope, scale, causal, lengths, past):

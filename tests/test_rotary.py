@@ -41,8 +41,8 @@ def check(out, x, positions, freqs, interleaved, offset, inverse, scale):
     bound = ref.abs() * step.eps / 2 + size * (16 * 2.0 ** -24 + far) \
         + step.tiny * step.eps
     assert out.dtype == x.dtype and out.shape == x.shape
-    assert ((out.double().cpu() - ref).abs() <= bound).all(), \
-        ((out.double().cpu() - ref).abs() / bound).max()
+    worst = ((out.double().cpu() - ref).abs() / bound).max().item()
+    assert worst <= 1.0
 
 
 @pytest.mark.parametrize("device", DEVICES)
