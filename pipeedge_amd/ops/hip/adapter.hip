@@ -38,6 +38,7 @@ struct InnerArgs {
     const float* scales;        // [n] or nullptr
     __bf16* inner;              // [M][rank_pad]
     int M, K, rows_per_id, n_adapters, rank, rank_pad;
+    int item_rows, item_blocks; // rows that blocks do not cross
     bool vec;                   // rows lie at multiples of 16 bytes
 };
 
@@ -164,6 +165,147 @@ __global__ __launch_bounds__(256) void adapter_inner_kernel(InnerArgs a) {
                 if (a.scales != nullptr) v *= a.scales[out_id];
             }
             a.inner[(long)out_row * a.rank_pad + col] = f2bf(v);
+        }
+    }
+}
+
+// The same through LDS, for so many rows that the operands' way into the
+// registers is the bound: fragments loaded straight from memory come in
+// pieces of 64 B, at a quarter of the rate of whole lines, and each wave
+// loads the adapters for itself. A block takes 32 WM rows by 32 WN inner
+// columns; WK groups of waves take a part of K each, in slices of 64 that are
+// loaded BUFS - 1 turns ahead of their use.
+template <int WN, int WM, int WK, int BUFS>
+__global__ __launch_bounds__(64 * WN * WM * WK)
+void adapter_inner_tile_kernel(InnerArgs a) {
+    constexpr int BN = 32 * WN, BM = 32 * WM, BK = 64, CH = BK / 8;
+    constexpr int SLICE = (BN + BM) * BK;
+    constexpr int PIECES = (BN + BM) / 8 / (WN * WM);
+    typedef TileVec<__bf16>::v8 v8;
+    __shared__ __attribute__((aligned(256))) __bf16 lds[WK * BUFS * SLICE];
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int l31 = lane & 31, hi = lane >> 5;
+    const int all = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wid = all % (WN * WM), wk = all / (WN * WM);
+    const int wn = wid % WN, wm = wid / WN;
+    const int item = blockIdx.x / a.item_blocks;
+    const int m0 = item * a.item_rows
+                   + (blockIdx.x - item * a.item_blocks) * BM;
+    const int end = min(m0 + BM, (item + 1) * a.item_rows);
+    const int n0 = blockIdx.y * BN;
+    __bf16* const smem = lds + wk * BUFS * SLICE;
+
+    // adapters of the block's rows, row l and l + 64 in lane l
+    int left[(BM + 63) / 64];
+    #pragma unroll
+    for (int i = 0; i < (BM + 63) / 64; ++i) {
+        const int r = i * 64 + lane;
+        const int v = r < BM && m0 + r < end
+            ? a.row_ids[(m0 + r) / a.rows_per_id] : -1;
+        left[i] = v < a.n_adapters ? v : -1;
+    }
+    const int row = m0 + wm * 32 + l31;
+    const int id = row < end ? a.row_ids[row / a.rows_per_id] : -1;
+    // slices of this part of K; all parts take as many turns
+    const int turns = ((a.K + BK - 1) / BK + WK - 1) / WK;
+    const int slice0 = wk * turns;
+    const int slices = min(turns, max(0, (a.K + BK - 1) / BK - slice0));
+    const auto fast = [&](int t) {
+        return a.vec && (slice0 + t + 1) * BK <= a.K;
+    };
+
+    while (true) {
+        int cur = -1;
+        #pragma unroll
+        for (int i = 0; i < (BM + 63) / 64; ++i) {
+            const unsigned long long has = __ballot(left[i] >= 0);
+            if (cur < 0 && has)
+                cur = __builtin_amdgcn_readlane(left[i],
+                                                __builtin_ctzll(has));
+        }
+        if (cur < 0) break;
+        #pragma unroll
+        for (int i = 0; i < (BM + 63) / 64; ++i)
+            if (left[i] == cur) left[i] = -1;
+        const __bf16* down = a.down + (long)cur * a.rank * a.K;
+
+        const auto stage = [&](int t) {
+            __bf16* image = smem + (t % BUFS) * SLICE;
+            #pragma unroll
+            for (int i = 0; i < PIECES; ++i) {
+                const int r = (wid * PIECES + i) * 8 + lane / CH;
+                const int c = (lane % CH) ^ tile_key<CH>(r);
+                const __bf16* from = r < BN
+                    ? down + (long)min(n0 + r, a.rank - 1) * a.K
+                    : a.x + (long)min(m0 + r - BN, end - 1) * a.K;
+                __bf16* to = image + (wid * PIECES + i) * 512;
+                const int k = (slice0 + t) * BK + c * 8;
+                if (fast(t))
+                    tile_load(from + k, to);
+                else
+                    *reinterpret_cast<bf16x8*>(to + lane * 8) =
+                        inner_load(from, k, a.K, a.vec);
+            }
+        };
+        f32x16 acc = {};
+        const unsigned base = tile_row_base<CH, 32>(tile_lds(smem), lane);
+        __syncthreads();
+        #pragma unroll
+        for (int t = 0; t < BUFS - 1; ++t)
+            if (t < slices) stage(t);
+        for (int t = 0; t < turns; ++t) {
+            // slice t is here; those behind it may be on their way
+            if (BUFS == 4 && t + 2 < slices && fast(t + 2))
+                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)"
+                             ::"i"(2 * PIECES) : "memory");
+            else if (t + 1 < slices && fast(t + 1))
+                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)"
+                             ::"i"(PIECES) : "memory");
+            else
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            // into the buffer that every wave left before the barrier
+            if (t + BUFS - 1 < slices) stage(t + BUFS - 1);
+            if (t >= slices) continue;
+            const unsigned at = base + (t % BUFS) * SLICE * 2;
+            #pragma unroll
+            for (int s = 0; s < BK / 16; ++s) {
+                const v8 d = tile_row_read<__bf16, CH, 32>(
+                    at + wn * 32 * BK * 2, 0, s);
+                const v8 x = tile_row_read<__bf16, CH, 32>(
+                    at + (BN + wm * 32) * BK * 2, 0, s);
+                acc = tile_mfma(d, x, acc);
+            }
+        }
+        if constexpr (WK > 1) {
+            // the parts of K meet in LDS, in their order
+            __syncthreads();
+            f32x16* sums = reinterpret_cast<f32x16*>(lds)
+                           + wid * 64 + lane;
+            static_assert(WN * WM * (WK - 1) * 64 * 64
+                          <= WK * BUFS * SLICE * 2, "room for the sums");
+            if (wk > 0) sums[(wk - 1) * WN * WM * 64] = acc;
+            __syncthreads();
+            if (wk == 0)
+                #pragma unroll
+                for (int p = 0; p < WK - 1; ++p)
+                    acc += sums[p * WN * WM * 64];
+        }
+        if (wk == 0 && id == cur) {
+            const float scale = a.scales != nullptr ? a.scales[cur] : 1.0f;
+            #pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int col = n0 + wn * 32 + g * 8 + hi * 4;
+                TileVec<__bf16>::v4 o;
+                #pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    o[j] = f2bf(col + j < a.rank ? acc[g * 4 + j] * scale
+                                                 : 0.0f);
+                *reinterpret_cast<TileVec<__bf16>::v4*>(
+                    a.inner + (long)row * a.rank_pad + col) = o;
+            }
         }
     }
 }
@@ -475,7 +617,10 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void adapter_product_kernel(
     // are done; behind the barrier that holds for all waves. LDS-DMA arrives
     // in order, so the pieces of later slices may stay on their way.
     const auto arrive = [&](int t) {
-        if (BUFS == 3 && t + 1 < staged && fast(t + 1))
+        if (BUFS == 4 && t + 2 < staged && fast(t + 2))
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"(2 * PIECES)
+                         : "memory");
+        else if (BUFS >= 3 && t + 1 < staged && fast(t + 1))
             asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"(PIECES)
                          : "memory");
         else
@@ -624,19 +769,21 @@ void product_launch(ProductArgs& a) {
                        pe_current_stream(), a);
 }
 
+// The largest tile that still fills most of the 256 CUs: larger tiles read
+// less through L2 for each product, but a CU without a block does nothing.
+// Measured without adapters, us, tiles in this order (columns by rows):
+//   8192 x 1024 -> 2048    41  47  55  59
+//   1576 x 1024 -> 4096    36  23  27  27
+//   1576 x 768  -> 2304    28  18  13  14
+//    512 x 1280 -> 1280    39  25  15  10
 void adapter_product(ProductArgs& a) {
-    static const int force = [] {
-        const char* s = std::getenv("PIPEEDGE_ADAPTER_T");
-        return s ? std::atoi(s) : 0;
-    }();
-    if (force == 1) product_launch<2, 4, 4, 2, 64, 2>(a);
-    else if (force == 2) product_launch<2, 2, 2, 2, 64, 2>(a);
-    else if (force == 3) product_launch<1, 1, 2, 2, 64, 2>(a);
-    else if (force == 4) product_launch<2, 4, 2, 2, 32, 3>(a);
-    else if (force == 5) product_launch<4, 2, 2, 2, 32, 3>(a);
-    else if (force == 6) product_launch<2, 2, 2, 2, 32, 3>(a);
-    else if (force == 7) product_launch<1, 1, 2, 2, 64, 3>(a);
-    else product_launch<2, 4, 2, 2, 32, 3>(a);
+    const auto blocks = [&](long columns, long rows) {
+        return ((a.N + columns - 1) / columns) * ((a.M + rows - 1) / rows);
+    };
+    if (blocks(256, 256) >= 200) product_launch<2, 4, 4, 2, 64, 2>(a);
+    else if (blocks(256, 128) >= 160) product_launch<2, 2, 4, 2, 64, 3>(a);
+    else if (blocks(128, 128) >= 128) product_launch<1, 2, 4, 2, 64, 3>(a);
+    else product_launch<1, 1, 2, 2, 64, 2>(a);
 }
 
 // Rows that the kernels for few rows take.
@@ -657,6 +804,25 @@ void adapter_inner(const InnerArgs& a) {
         hipLaunchKernelGGL(adapter_inner_step_kernel,
                            dim3(a.M, a.rank_pad / 16), dim3(256), 0,
                            pe_current_stream(), a);
+        return;
+    }
+    // From about 2048 rows of rank 64 on, the way through LDS wins (12608
+    // rows of 1280: rank 64 26 us against 10, rank 16 12 against 11; 3152
+    // rows: rank 64 10 against 9; 1576 rows of 768, rank 8: 4.5 against 12).
+    if ((long)a.M * a.rank_pad >= 2048L * 64 * (a.rank <= 32 ? 2 : 1)) {
+        InnerArgs t = a;
+        // blocks that end with their item have one adapter and read K once
+        t.item_rows = a.rows_per_id >= 64 ? a.rows_per_id : a.M;
+        t.item_blocks = (t.item_rows + 63) / 64;
+        const int rows = t.item_blocks * (a.M / t.item_rows);
+        if (a.rank <= 32)
+            hipLaunchKernelGGL((adapter_inner_tile_kernel<1, 2, 2, 4>),
+                               dim3(rows, 1), dim3(256), 0,
+                               pe_current_stream(), t);
+        else
+            hipLaunchKernelGGL((adapter_inner_tile_kernel<2, 2, 2, 4>),
+                               dim3(rows, a.rank_pad / 64), dim3(512), 0,
+                               pe_current_stream(), t);
         return;
     }
     // columns a block: all of them up to 64, then 64 at a time
@@ -770,7 +936,7 @@ torch::Tensor adapter_linear_op(
         t = adapter_dense(*t);
         return reinterpret_cast<const __bf16*>(t->data_ptr());
     };
-    const int rank_pad = (r + 31) / 32 * 32;
+    const int rank_pad = r <= 32 ? 32 : (r + 63) / 64 * 64;
     const bool any = n > 0 && r > 0;
     auto inner = torch::empty({any ? M : 0, rank_pad}, x.options());
     auto out = torch::empty(out_sizes, x.options());
