@@ -71,8 +71,8 @@ __device__ __forceinline__ int wave_scan(int v, int lane) {
     return v;
 }
 
-__device__ __forceinline__ long cache_total(const CacheArgs& a, int lane) {
-    long total = 0;
+__device__ __forceinline__ int cache_total(const CacheArgs& a, int lane) {
+    int total = 0;
     for (int b0 = 0; b0 < a.B; b0 += 64)
         total += __builtin_amdgcn_readlane(
             wave_scan(cache_tiles(a, b0 + lane), lane), 63);
@@ -81,36 +81,43 @@ __device__ __forceinline__ long cache_total(const CacheArgs& a, int lane) {
 
 // Place of tile number `at` (of all row groups and sequences): the sequence
 // and the number of its first tile.
-__device__ __forceinline__ void cache_find(const CacheArgs& a, long at,
-                                           int lane, int& seq, long& first) {
-    long before = 0;
+__device__ __forceinline__ void cache_find(const CacheArgs& a, int at,
+                                           int lane, int& seq, int& first) {
+    int before = 0;
     for (int b0 = 0; b0 < a.B; b0 += 64) {
         const int mine = cache_tiles(a, b0 + lane);
         const int upto = wave_scan(mine, lane);
-        const long end = before + (long)upto * a.row_groups;
+        const int end = before + upto * a.row_groups;
         const unsigned long long past = __ballot(end > at);
         if (past) {
             const int l = __builtin_ctzll(past);
             seq = b0 + l;
-            first = before + (long)(__builtin_amdgcn_readlane(upto, l)
+            first = before + (__builtin_amdgcn_readlane(upto, l)
                      - __builtin_amdgcn_readlane(mine, l)) * a.row_groups;
             return;
         }
-        before += (long)__builtin_amdgcn_readlane(upto, 63) * a.row_groups;
+        before += __builtin_amdgcn_readlane(upto, 63) * a.row_groups;
     }
     seq = a.B;
     first = before;
 }
 
 // tiles of block g: run_start(g) .. run_start(g + 1)
-__device__ __forceinline__ long run_start(long total, int g, int blocks) {
-    return total / blocks * g + min((long)g, total % blocks);
+__device__ __forceinline__ int run_start(int total, int g, int blocks) {
+    return total / blocks * g + min(g, total % blocks);
 }
 // the block that has tile `at`
-__device__ __forceinline__ int run_block(long total, long at, int blocks) {
-    const long each = total / blocks, extra = total % blocks;
-    if (at < extra * (each + 1)) return (int)(at / (each + 1));
-    return (int)(extra + (at - extra * (each + 1)) / each);
+__device__ __forceinline__ int run_block(int total, int at, int blocks) {
+    const int each = total / blocks, extra = total % blocks;
+    if (at < extra * (each + 1)) return at / (each + 1);
+    return extra + (at - extra * (each + 1)) / each;
+}
+
+// The accumulators take one half of the register file. Arithmetic on them in
+// a rare branch would make the compiler carry them in the other half and copy
+// them back and forth in every tile.
+__device__ __forceinline__ void keep_in_agprs(f32x4& v) {
+    asm volatile("" : "+a"(v));
 }
 
 // Where the 8 tokens of one group lie: the address of the first, and the
@@ -123,8 +130,11 @@ struct CacheGroup {
 
 // WR groups of 16 rows times WT waves a group, KEYS / WT tokens each.
 template <typename T, int R, int DR, int WR, int WT>
-__global__ __launch_bounds__(64 * WR * WT, 2)
+__global__ __launch_bounds__(64 * WR * WT, WR * WT > 4 ? 2 : 1)
 void latent_cache_kernel(CacheArgs a) {
+    // one wave on a SIMD has 512 registers, one of two has 256
+    constexpr bool ONE = WR * WT <= 4;
+    constexpr int AHEAD = ONE ? 8 : 2;
     constexpr int CL = R / 8, CR = DR / 8;      // chunks of a row's parts
     constexpr int NT = R / 16;                  // output tiles
     constexpr int TOKENS = KEYS / WT;           // tokens a wave and tile
@@ -147,22 +157,22 @@ void latent_cache_kernel(CacheArgs a) {
     T* const images = smem + share * 2 * TILE;
     const unsigned lds = tile_lds(images);
 
-    const long total = cache_total(a, lane);
-    long at = run_start(total, blockIdx.x, gridDim.x);
-    const long end = run_start(total, blockIdx.x + 1, gridDim.x);
+    const int total = cache_total(a, lane);
+    const int block = xcd_contiguous(blockIdx.x, gridDim.x);
+    int at = run_start(total, block, gridDim.x);
+    const int end = run_start(total, block + 1, gridDim.x);
     if (at >= end) return;
-    int seq;
-    long first;
+    int seq, first;
     cache_find(a, at, lane, seq, first);
 
     while (at < end) {
         const int len = cache_length(a, seq);
         const int tiles = (len + KEYS - 1) / KEYS;
         if (tiles == 0) { ++seq; continue; }
-        const int rg = (int)((at - first) / tiles);
-        const long base = first + (long)rg * tiles;
-        const int t0 = (int)(at - base);
-        const int t1 = (int)min((long)tiles, end - base);
+        const int rg = (at - first) / tiles;
+        const int base = first + rg * tiles;
+        const int t0 = at - base;
+        const int t1 = min(tiles, end - base);
 
         // this lane's row and the last token that it sees
         const int row = (rg * WR + group) * 16 + l15;
@@ -291,19 +301,46 @@ void latent_cache_kernel(CacheArgs a) {
             const int tok0 = t * KEYS + share * TOKENS;
 
             if (live) {
+            // Operands are read from LDS a batch ahead of their MFMAs: one
+            // wave on a SIMD has nothing else to wait with.
             f32x4 s[SUB] = {};
+            v8 f[2][AHEAD];
+            const auto key = [&](int j) {
+                const int i = j / SUB, m = j % SUB;
+                return i < R / 32
+                    ? tile_row_read<T, CL, 16>(latent, m * 16, i)
+                    : tile_row_read<T, CR, 16>(rope, m * 16, i - R / 32);
+            };
+            const auto val = [&](int j) {
+                return tile_column_read<T, CL, 16>(value, j / NT * 32,
+                                                   j % NT);
+            };
+            constexpr int KF = SUB * (R + DR) / 32, VF = SUB / 2 * NT;
+            constexpr int KB = (KF + AHEAD - 1) / AHEAD;
+            constexpr int VB = VF / AHEAD;
+            static_assert(VF % AHEAD == 0, "whole batches");
             #pragma unroll
-            for (int i = 0; i < R / 32; ++i)
-                #pragma unroll
-                for (int m = 0; m < SUB; ++m)
-                    s[m] = tile_mfma(tile_row_read<T, CL, 16>(
-                        latent, m * 16, i), bq[i], s[m]);
+            for (int j = 0; j < AHEAD; ++j) f[0][j] = key(j);
             #pragma unroll
-            for (int i = 0; i < DR / 32; ++i)
+            for (int b = 0; b < KB; ++b) {
                 #pragma unroll
-                for (int m = 0; m < SUB; ++m)
-                    s[m] = tile_mfma(tile_row_read<T, CR, 16>(
-                        rope, m * 16, i), bq[R / 32 + i], s[m]);
+                for (int j = 0; j < AHEAD; ++j)
+                    if ((b + 1) * AHEAD + j < KF)
+                        f[(b + 1) & 1][j] = key((b + 1) * AHEAD + j);
+                __builtin_amdgcn_sched_barrier(0);
+                #pragma unroll
+                for (int j = 0; j < AHEAD; ++j) {
+                    const int k = b * AHEAD + j;
+                    if (k < KF)
+                        s[k % SUB] = tile_mfma(f[b & 1][j], bq[k / SUB],
+                                               s[k % SUB]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            // the first values, while the weights are formed
+            #pragma unroll
+            for (int j = 0; j < AHEAD; ++j) f[0][j] = val(j);
+            __builtin_amdgcn_sched_barrier(0);
 
             if (__any(limit < tok0 + TOKENS - 1)) {
                 #pragma unroll
@@ -328,9 +365,11 @@ void latent_cache_kernel(CacheArgs a) {
                 sub = next == -INFINITY ? 0.0f : next - softmax::BIAS;
                 sum *= turn;
                 #pragma unroll
-                for (int n = 0; n < NT; ++n)
-                    #pragma unroll
-                    for (int i = 0; i < 4; ++i) acc[n][i] *= turn;
+                for (int n = 0; n < NT; ++n) {
+                    if constexpr (ONE) keep_in_agprs(acc[n]);
+                    acc[n] *= turn;
+                    if constexpr (ONE) keep_in_agprs(acc[n]);
+                }
             }
             #pragma unroll
             for (int m = 0; m < SUB; ++m)
@@ -340,16 +379,28 @@ void latent_cache_kernel(CacheArgs a) {
                         fmaf(s[m][i], a.scale, -sub));
                     sum += s[m][i];
                 }
+            v8 w[SUB / 2];
             #pragma unroll
             for (int m = 0; m < SUB; m += 2) {
                 float p[8];
                 #pragma unroll
                 for (int j = 0; j < 8; ++j) p[j] = s[m + j / 4][j % 4];
-                const v8 w = tile_weights<T>(p);
+                w[m / 2] = tile_weights<T>(p);
+            }
+            #pragma unroll
+            for (int b = 0; b < VB; ++b) {
                 #pragma unroll
-                for (int n = 0; n < NT; ++n)
-                    acc[n] = tile_mfma(tile_column_read<T, CL, 16>(
-                        value, m * 16, n), w, acc[n]);
+                for (int j = 0; j < AHEAD; ++j)
+                    if (b + 1 < VB)
+                        f[(b + 1) & 1][j] = val((b + 1) * AHEAD + j);
+                __builtin_amdgcn_sched_barrier(0);
+                #pragma unroll
+                for (int j = 0; j < AHEAD; ++j) {
+                    const int k = b * AHEAD + j;
+                    acc[k % NT] = tile_mfma(f[b & 1][j], w[k / NT],
+                                            acc[k % NT]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
             }
             }
             if (ALONE && t + 2 < t1) stage(t + 2, t & 1);
@@ -412,10 +463,9 @@ void latent_cache_kernel(CacheArgs a) {
                         out + n * 16) = o;
                 }
             } else {
-                // block and work item numbers only grow together, so their
+                // run and work item numbers only grow together, so their
                 // sum is a slot that no other segment has
-                const long slot = (long)blockIdx.x
-                    + (long)seq * a.row_groups + rg;
+                const long slot = (long)block + (long)seq * a.row_groups + rg;
                 const long at_row = slot * (16 * WR) + group * 16 + l15;
                 float* out = a.part + at_row * R + quad * 4;
                 #pragma unroll
@@ -426,7 +476,7 @@ void latent_cache_kernel(CacheArgs a) {
         }
         at = base + t1;
         if (t1 == tiles && rg + 1 == a.row_groups) {
-            first += (long)tiles * a.row_groups;
+            first += tiles * a.row_groups;
             ++seq;
         }
     }
@@ -453,7 +503,7 @@ __global__ __launch_bounds__(256) void latent_cache_join_kernel(
         return;
     }
     const int rg = row / block_rows;
-    long total = 0, first = 0;
+    int total = 0, first = 0;
     for (int b0 = 0; b0 < a.B; b0 += 64) {
         const int mine = cache_tiles(a, b0 + lane);
         const int upto = wave_scan(mine, lane);
@@ -462,25 +512,38 @@ __global__ __launch_bounds__(256) void latent_cache_join_kernel(
         total += __builtin_amdgcn_readlane(upto, 63);
     }
     total *= a.row_groups;
-    first = first * a.row_groups + (long)rg * tiles;
+    first = first * a.row_groups + rg * tiles;
     const int g0 = run_block(total, first, blocks);
     const int g1 = run_block(total, first + tiles - 1, blocks);
     if (g0 == g1) return;
-    const long slot0 = (long)seq * a.row_groups + rg;
-    const int r = row - rg * block_rows;
+    const long row0 = ((long)seq * a.row_groups + rg) * block_rows
+                      + row - rg * block_rows;
+    // lane l has the statistics of segments l, l + 64, ..
     float top = -INFINITY;
-    for (int g = g0; g <= g1; ++g)
-        top = fmaxf(top, a.part_stat[(slot0 + g) * block_rows + r].x);
+    for (int g = g0 + lane; g <= g1; g += 64)
+        top = fmaxf(top, a.part_stat[row0 + (long)g * block_rows].x);
+    top = wave64_reduce(top, MaxOp());
     float sum = 0.0f;
     vec acc = {};
-    for (int g = g0; g <= g1; ++g) {
-        const long at = (slot0 + g) * block_rows + r;
-        const float2 st = a.part_stat[at];
-        const float f = st.x == -INFINITY
+    for (int h0 = g0; h0 <= g1; h0 += 64) {
+        const int g = min(h0 + lane, g1);
+        const float2 st = a.part_stat[row0 + (long)g * block_rows];
+        const float f = st.x == -INFINITY || h0 + lane > g1
             ? 0.0f : __builtin_amdgcn_exp2f(st.x - top);
-        sum += st.y == st.y ? st.y * f : st.y;
-        acc += *reinterpret_cast<const vec*>(a.part + at * R + lane * E) * f;
+        // a total that is not a number stays one, whatever its reference
+        sum += h0 + lane > g1 ? 0.0f : st.y == st.y ? st.y * f : st.y;
+        const int count = min(64, g1 - h0 + 1);
+        #pragma unroll 4
+        for (int i = 0; i < count; ++i) {
+            const float fi = __builtin_bit_cast(
+                float, __builtin_amdgcn_readlane(
+                    __builtin_bit_cast(int, f), i));
+            acc += *reinterpret_cast<const vec*>(
+                a.part + (row0 + (long)(h0 + i) * block_rows) * R + lane * E)
+                * fi;
+        }
     }
+    sum = wave64_reduce(sum, SumOp());
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     ovec o;
     #pragma unroll
@@ -507,8 +570,7 @@ void cache_launch_shape(const CacheArgs& a, int blocks) {
 
 template <typename T, int R, int DR>
 void cache_launch(const CacheArgs& a, int block_rows, int blocks) {
-    if (block_rows == 128) cache_launch_shape<T, R, DR, 8, 1>(a, blocks);
-    else if (block_rows == 64) cache_launch_shape<T, R, DR, 4, 2>(a, blocks);
+    if (block_rows == 64) cache_launch_shape<T, R, DR, 4, 1>(a, blocks);
     else if (block_rows == 32) cache_launch_shape<T, R, DR, 2, 2>(a, blocks);
     else cache_launch_shape<T, R, DR, 1, 2>(a, blocks);
 }
@@ -607,12 +669,13 @@ torch::Tensor latent_cache_attention_op(
     a.B = B, a.H = H, a.Sq = Sq, a.table_width = width;
     a.rows = Sq * H;
     a.scale = scale * 1.4426950408889634;
-    const int block_rows = a.rows <= 16 ? 16 : a.rows <= 32 ? 32
-                           : a.rows <= 64 ? 64 : 128;
+    const int block_rows = a.rows <= 16 ? 16 : a.rows <= 32 ? 32 : 64;
     a.row_groups = (a.rows + block_rows - 1) / block_rows;
     // LDS holds one block a CU; no more blocks than there can be tiles
     const int64_t items = B * a.row_groups;
     const int64_t most = items * ((page * width + KEYS - 1) / KEYS);
+    TORCH_CHECK_VALUE(most < (1L << 31) - 512,
+                      "latent_cache_attention: too many tokens");
     const int blocks = std::min<int64_t>(256, most);
     const int64_t slots = items + blocks;
     auto part = torch::empty({slots * block_rows * (latent_dim + 2)},
