@@ -6,13 +6,15 @@
 // pass over the cache serves all heads; 16 heads are bound by memory, 128 by
 // the matrix cores.
 //
-// Work is cut into tiles of 64 cached tokens, numbered through all sequences
-// and row groups, and each of a fixed number of blocks takes an equal run of
-// them, across sequences where it falls so: lengths stay on the device, and
-// ragged batches are balanced to within a tile. A run inside one (sequence,
-// row group) is a segment; a segment that covers all its tiles is written to
-// the output, others leave partial sums in fp32 that a second kernel joins
-// in a fixed order.
+// Work is cut into tiles of 64 cached tokens, numbered through all sequences,
+// and a fixed number of runs takes an equal share of them, across sequences
+// where it falls so: lengths stay on the device, and ragged batches are
+// balanced to within a tile. A run has a block for each group of rows; they
+// are neighbours on one XCD and walk over the same tiles at the same time, so
+// that one of them fetches a tile from memory and the others find it in L2.
+// A run's part of one sequence is a segment; a segment that covers all tiles
+// is written to the output, others leave partial sums in fp32 that a second
+// kernel joins in a fixed order.
 //
 // Both products are transposed as in the expanded form, on 16x16x32 MFMAs: a
 // wave owns 16 rows, a lane holds one row's scores, and the weights are the
@@ -48,7 +50,7 @@ struct CacheArgs {
     bool page_of_groups;            // a multiple of 8 tokens
     int B, H, Sq, table_width;
     int rows;                       // Sq * H
-    int row_groups;                 // ceil(rows / rows a block)
+    int row_groups, runs;           // ceil(rows / rows a block)
     float scale;                    // times log2(e)
 };
 
@@ -76,39 +78,38 @@ __device__ __forceinline__ int cache_total(const CacheArgs& a, int lane) {
     for (int b0 = 0; b0 < a.B; b0 += 64)
         total += __builtin_amdgcn_readlane(
             wave_scan(cache_tiles(a, b0 + lane), lane), 63);
-    return total * a.row_groups;
+    return total;
 }
 
-// Place of tile number `at` (of all row groups and sequences): the sequence
-// and the number of its first tile.
+// Place of tile number `at`: the sequence and the number of its first tile.
 __device__ __forceinline__ void cache_find(const CacheArgs& a, int at,
                                            int lane, int& seq, int& first) {
     int before = 0;
     for (int b0 = 0; b0 < a.B; b0 += 64) {
         const int mine = cache_tiles(a, b0 + lane);
         const int upto = wave_scan(mine, lane);
-        const int end = before + upto * a.row_groups;
+        const int end = before + upto;
         const unsigned long long past = __ballot(end > at);
         if (past) {
             const int l = __builtin_ctzll(past);
             seq = b0 + l;
-            first = before + (__builtin_amdgcn_readlane(upto, l)
-                     - __builtin_amdgcn_readlane(mine, l)) * a.row_groups;
+            first = before + __builtin_amdgcn_readlane(upto, l)
+                    - __builtin_amdgcn_readlane(mine, l);
             return;
         }
-        before += __builtin_amdgcn_readlane(upto, 63) * a.row_groups;
+        before += __builtin_amdgcn_readlane(upto, 63);
     }
     seq = a.B;
     first = before;
 }
 
-// tiles of block g: run_start(g) .. run_start(g + 1)
-__device__ __forceinline__ int run_start(int total, int g, int blocks) {
-    return total / blocks * g + min(g, total % blocks);
+// tiles of run g: run_start(g) .. run_start(g + 1)
+__device__ __forceinline__ int run_start(int total, int g, int runs) {
+    return total / runs * g + min(g, total % runs);
 }
-// the block that has tile `at`
-__device__ __forceinline__ int run_block(int total, int at, int blocks) {
-    const int each = total / blocks, extra = total % blocks;
+// the run that has tile `at`
+__device__ __forceinline__ int run_of(int total, int at, int runs) {
+    const int each = total / runs, extra = total % runs;
     if (at < extra * (each + 1)) return at / (each + 1);
     return extra + (at - extra * (each + 1)) / each;
 }
@@ -159,8 +160,9 @@ void latent_cache_kernel(CacheArgs a) {
 
     const int total = cache_total(a, lane);
     const int block = xcd_contiguous(blockIdx.x, gridDim.x);
-    int at = run_start(total, block, gridDim.x);
-    const int end = run_start(total, block + 1, gridDim.x);
+    const int run = block / a.row_groups, rg = block - run * a.row_groups;
+    int at = run_start(total, run, a.runs);
+    const int end = run_start(total, run + 1, a.runs);
     if (at >= end) return;
     int seq, first;
     cache_find(a, at, lane, seq, first);
@@ -169,10 +171,8 @@ void latent_cache_kernel(CacheArgs a) {
         const int len = cache_length(a, seq);
         const int tiles = (len + KEYS - 1) / KEYS;
         if (tiles == 0) { ++seq; continue; }
-        const int rg = (at - first) / tiles;
-        const int base = first + rg * tiles;
-        const int t0 = at - base;
-        const int t1 = min(tiles, end - base);
+        const int t0 = at - first;
+        const int t1 = min(tiles, end - first);
 
         // this lane's row and the last token that it sees
         const int row = (rg * WR + group) * 16 + l15;
@@ -463,9 +463,9 @@ void latent_cache_kernel(CacheArgs a) {
                         out + n * 16) = o;
                 }
             } else {
-                // run and work item numbers only grow together, so their
+                // run and sequence numbers only grow together, so their
                 // sum is a slot that no other segment has
-                const long slot = (long)block + (long)seq * a.row_groups + rg;
+                const long slot = (long)(run + seq) * a.row_groups + rg;
                 const long at_row = slot * (16 * WR) + group * 16 + l15;
                 float* out = a.part + at_row * R + quad * 4;
                 #pragma unroll
@@ -474,9 +474,9 @@ void latent_cache_kernel(CacheArgs a) {
                 if (quad == 0) a.part_stat[at_row] = make_float2(top, sum);
             }
         }
-        at = base + t1;
-        if (t1 == tiles && rg + 1 == a.row_groups) {
-            first += tiles * a.row_groups;
+        at = first + t1;
+        if (t1 == tiles) {
+            first += tiles;
             ++seq;
         }
     }
@@ -487,7 +487,7 @@ void latent_cache_kernel(CacheArgs a) {
 // hold nothing get zeros; whole segments are there already.
 template <typename T, int R>
 __global__ __launch_bounds__(256) void latent_cache_join_kernel(
-        CacheArgs a, int block_rows, int blocks) {
+        CacheArgs a, int block_rows) {
     constexpr int E = R / 64;                   // elements a lane
     typedef float vec __attribute__((ext_vector_type(E)));
     typedef T ovec __attribute__((ext_vector_type(E)));
@@ -502,7 +502,6 @@ __global__ __launch_bounds__(256) void latent_cache_join_kernel(
         *reinterpret_cast<ovec*>(out) = ovec{};
         return;
     }
-    const int rg = row / block_rows;
     int total = 0, first = 0;
     for (int b0 = 0; b0 < a.B; b0 += 64) {
         const int mine = cache_tiles(a, b0 + lane);
@@ -511,23 +510,22 @@ __global__ __launch_bounds__(256) void latent_cache_join_kernel(
             first = total + __builtin_amdgcn_readlane(upto, seq - b0) - tiles;
         total += __builtin_amdgcn_readlane(upto, 63);
     }
-    total *= a.row_groups;
-    first = first * a.row_groups + rg * tiles;
-    const int g0 = run_block(total, first, blocks);
-    const int g1 = run_block(total, first + tiles - 1, blocks);
+    const int g0 = run_of(total, first, a.runs);
+    const int g1 = run_of(total, first + tiles - 1, a.runs);
     if (g0 == g1) return;
-    const long row0 = ((long)seq * a.row_groups + rg) * block_rows
-                      + row - rg * block_rows;
+    // row of segment g: row0 + g * step
+    const long step = (long)a.row_groups * block_rows;
+    const long row0 = seq * step + row;
     // lane l has the statistics of segments l, l + 64, ..
     float top = -INFINITY;
     for (int g = g0 + lane; g <= g1; g += 64)
-        top = fmaxf(top, a.part_stat[row0 + (long)g * block_rows].x);
+        top = fmaxf(top, a.part_stat[row0 + g * step].x);
     top = wave64_reduce(top, MaxOp());
     float sum = 0.0f;
     vec acc = {};
     for (int h0 = g0; h0 <= g1; h0 += 64) {
         const int g = min(h0 + lane, g1);
-        const float2 st = a.part_stat[row0 + (long)g * block_rows];
+        const float2 st = a.part_stat[row0 + g * step];
         const float f = st.x == -INFINITY || h0 + lane > g1
             ? 0.0f : __builtin_amdgcn_exp2f(st.x - top);
         // a total that is not a number stays one, whatever its reference
@@ -539,7 +537,7 @@ __global__ __launch_bounds__(256) void latent_cache_join_kernel(
                 float, __builtin_amdgcn_readlane(
                     __builtin_bit_cast(int, f), i));
             acc += *reinterpret_cast<const vec*>(
-                a.part + (row0 + (long)(h0 + i) * block_rows) * R + lane * E)
+                a.part + (row0 + (h0 + i) * step) * R + lane * E)
                 * fi;
         }
     }
@@ -565,7 +563,7 @@ void cache_launch_shape(const CacheArgs& a, int blocks) {
                        dim3(64 * WR * WT), 0, pe_current_stream(), a);
     hipLaunchKernelGGL((latent_cache_join_kernel<T, R>),
                        dim3((a.rows + 3) / 4, a.B), dim3(256), 0,
-                       pe_current_stream(), a, 16 * WR, blocks);
+                       pe_current_stream(), a, 16 * WR);
 }
 
 template <typename T, int R, int DR>
@@ -671,13 +669,13 @@ torch::Tensor latent_cache_attention_op(
     a.scale = scale * 1.4426950408889634;
     const int block_rows = a.rows <= 16 ? 16 : a.rows <= 32 ? 32 : 64;
     a.row_groups = (a.rows + block_rows - 1) / block_rows;
-    // LDS holds one block a CU; no more blocks than there can be tiles
-    const int64_t items = B * a.row_groups;
-    const int64_t most = items * ((page * width + KEYS - 1) / KEYS);
+    // LDS holds one block a CU; no more runs than there can be tiles
+    const int64_t most = B * ((page * width + KEYS - 1) / KEYS);
     TORCH_CHECK_VALUE(most < (1L << 31) - 512,
                       "latent_cache_attention: too many tokens");
-    const int blocks = std::min<int64_t>(256, most);
-    const int64_t slots = items + blocks;
+    a.runs = std::min<int64_t>(std::max(256 / a.row_groups, 1), most);
+    const int blocks = a.runs * a.row_groups;
+    const int64_t slots = (B + a.runs) * a.row_groups;
     auto part = torch::empty({slots * block_rows * (latent_dim + 2)},
                              q.options().dtype(torch::kFloat));
     a.part = part.data_ptr<float>();

@@ -39,25 +39,28 @@ __device__ __forceinline__ f32x4 tile_mfma(TileVec<_Float16>::v8 a,
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-// An LDS image holds rows (tokens) of CH 16-byte chunks without padding, as
-// LDS-DMA writes it; chunk c of row r lies at chunk position c ^ key(r). The
-// key makes both reads free of bank conflicts (64 banks of 4 B; 256 B, 16 or
-// 32 lanes, a cycle):
-// - 16 consecutive rows at one chunk (the score product's operand),
-// - 4 or 8 consecutive rows at 2 or 4 adjacent chunks (the transposing reads
-//   of the value product).
-// Rows of 16k chunks all start at bank 0, so 16 keys are needed: the low two
-// bits of the row choose among groups of 4 chunks, the third among pairs.
-// Rows of 16k + 8 chunks alternate between two halves already, rows of
-// 8k + 4 between four quarters.
+// An LDS image holds rows of CH 16-byte chunks without padding, as LDS-DMA
+// writes it; chunk c of row r lies at chunk position c ^ key(r). The key keeps
+// both reads at full rate (64 banks of 4 B, 256 B a cycle):
+// - rows at one chunk (M = 32) or at 4 adjacent ones (M = 16, the chunk from
+//   lane / 16). A 16-byte read takes 16 lanes a cycle, 0-3, 12-15 and 20-27
+//   of the first 32, then the other 16, so for M = 16 rows 0-3 and 12-15 at
+//   one chunk meet rows 4-11 at the next one: the second lowest key bit tells
+//   these row sets apart, and the lowest one is free to pair rows in a set
+//   (124 B a cycle with the row's bits in order, 230 so);
+// - 8 consecutive rows at 2 or 4 adjacent chunks (the transposing reads).
+// Rows of 16k chunks all start at bank 0, so the low two bits of the row
+// choose among groups of 4 chunks; rows of 16k + 8 chunks alternate between
+// two halves already, rows of 8k + 4 between four quarters.
 template <int CH>
 __device__ __forceinline__ constexpr int tile_key(int row) {
+    const int low = (((row >> 3) ^ (row >> 2)) & 1) * 2 + ((row >> 3) & 1);
     if constexpr (CH % 16 == 0)
-        return ((row & 3) << 2) | (((row >> 2) & 1) << 1) | ((row >> 3) & 1);
+        return ((row & 3) << 2) | low;
     else if constexpr (CH % 8 == 0)
-        return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
+        return (((row >> 1) & 1) << 2) | low;
     else
-        return (row >> 2) & 3;
+        return low;
 }
 
 // 16 bytes a lane from global memory into LDS at base + lane * 16
@@ -138,7 +141,7 @@ __device__ __forceinline__ typename TileVec<T>::v8 tile_column_read(
         unsigned base, int row0, int n) {
     constexpr int G = tile_group<CH>(), STEP = M / 8;
     constexpr int NEXT = 256 / M;       // rows to the second read
-    // 16 rows on, a row's key is the same; 8 rows on, one bit differs
+    // 16 rows on, a row's key is the same; 8 rows on, the same bits differ
     constexpr unsigned flip8 =
         NEXT == 16 ? 0 : (tile_key<CH>(8) ^ tile_key<CH>(0)) << 4;
     const unsigned flip = (STEP * n % G) << 4;
