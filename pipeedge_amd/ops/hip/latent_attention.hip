@@ -115,6 +115,8 @@ __global__ __launch_bounds__(256, 2) void latent_attention_kernel(
 
     const unsigned lds = tile_lds(smem);
     if (tiles > 0) stage(0, 0);
+    #pragma unroll
+    for (int i = 0; i < (DN + DR) / 16; ++i) tile_settle(bq[i]);
     for (int t = 0; t < tiles; ++t) {
         const unsigned image = lds + (t & 1) * TILE * 2;
         const unsigned nope = tile_row_base<CN, 32>(image, lane);

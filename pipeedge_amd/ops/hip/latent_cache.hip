@@ -34,8 +34,6 @@
 
 namespace {
 
-constexpr int KEYS = 64;            // tokens a tile
-
 struct CacheArgs {
     const void* q;                  // [B, Sq, H, R + DR]
     const void* cache;              // [pages, page size, R + DR]
@@ -47,11 +45,11 @@ struct CacheArgs {
     long q_b, q_s, q_h, c_p, c_t, t_b;      // strides in elements
     long pages;
     int page_size, page_shift;      // shift -1: not a power of two
-    bool page_of_groups;            // a multiple of 8 tokens
     int B, H, Sq, table_width;
     int rows;                       // Sq * H
     int row_groups;                 // ceil(rows / rows a block)
     int runs, least;                // most runs, fewest tiles of one
+    int tile_shift;                 // tokens a tile: 32 or 64
     float scale;                    // times log2(e)
 };
 
@@ -70,7 +68,8 @@ __device__ __forceinline__ int cache_length(const CacheArgs& a, int b) {
     return (int)min((long)max(as_constant(a.lengths)[b], 0), most);
 }
 __device__ __forceinline__ int cache_tiles(const CacheArgs& a, int b) {
-    return b < a.B ? (cache_length(a, b) + KEYS - 1) / KEYS : 0;
+    return b < a.B
+        ? (cache_length(a, b) + (1 << a.tile_shift) - 1) >> a.tile_shift : 0;
 }
 
 __device__ __forceinline__ int wave_scan(int v, int lane) {
@@ -143,8 +142,10 @@ struct CacheGroup {
     int last;
 };
 
-// WR groups of 16 rows times WT waves a group, KEYS / WT tokens each.
-template <typename T, int R, int DR, int WR, int WT>
+// WR groups of 16 rows times WT waves a group, each with its 32 tokens of a
+// tile.
+// GROUPED: pages hold whole groups of 8 tokens.
+template <typename T, int R, int DR, int WR, int WT, bool GROUPED>
 __global__ __launch_bounds__(64 * WR * WT, WR * WT > 4 ? 2 : 1)
 void latent_cache_kernel(CacheArgs a) {
     // one wave on a SIMD has 512 registers, one of two has 256
@@ -152,24 +153,28 @@ void latent_cache_kernel(CacheArgs a) {
     constexpr int AHEAD = ONE ? 8 : 2;
     constexpr int CL = R / 8, CR = DR / 8;      // chunks of a row's parts
     constexpr int NT = R / 16;                  // output tiles
-    constexpr int TOKENS = KEYS / WT;           // tokens a wave and tile
+    constexpr int TOKENS = 32, KEYS = TOKENS * WT;  // a wave's, a tile's
     constexpr int SUB = TOKENS / 16;            // score columns
     constexpr int GROUPS = TOKENS / 8 / WR;     // 8 tokens each, to load
     constexpr int TILE = TOKENS * (R + DR);
     // the waves of one row group load and use their tokens alone
     constexpr bool ALONE = WR == 1;
-    constexpr int PIECES = GROUPS * CL / 8 + GROUPS * CR / 8;
+    // Buffers of a share, and how many tiles its loads run ahead: where waves
+    // share tiles, behind the barrier that ends a buffer's use; a wave alone
+    // loads after its own use of the buffer.
+    constexpr int BUFS = WT == 1 ? 4 : 2, LEAD = ALONE ? 2 : BUFS - 1;
+    constexpr int PIECES = GROUPS * CL / 8 + (GROUPS * CR + 7) / 8;
     static_assert(!ALONE || (GROUPS == 4 && PIECES < 64), "counted waits");
     typedef typename TileVec<T>::v8 v8;
     typedef RunningTop<T> softmax;
-    // WT shares of two buffers of [latent | rope] images
-    __shared__ __attribute__((aligned(256))) T smem[WT * 2 * TILE];
+    // buffers of [latent | rope] images
+    __shared__ __attribute__((aligned(256))) T smem[WT * BUFS * TILE];
 
     const int tid = threadIdx.x;
     const int lane = tid & 63, l15 = lane & 15, quad = lane >> 4;
     const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int group = wid % WR, share = wid / WR;
-    T* const images = smem + share * 2 * TILE;
+    T* const images = smem + share * BUFS * TILE;
     const unsigned lds = tile_lds(images);
 
     int total, seq, first;
@@ -238,30 +243,19 @@ void latent_cache_kernel(CacheArgs a) {
             return page * a.c_p * 2
                    + (long)(tok - slot * a.page_size) * a.c_t * 2;
         };
-        long ahead = a.page_of_groups ? 0 : locate(t0);
-        const auto stage = [&](int t, int buf) {
-            T* image = images + buf * TILE + group * GROUPS * 8 * R;
-            T* rotary = images + buf * TILE + TOKENS * R
-                        + group * GROUPS * 8 * DR;
-            const int tok0 = t * KEYS + share * TOKENS + group * GROUPS * 8;
-            // piece p of the latent part has rows p * PR .. of this wave's
-            // tokens, of the rotary part rows p * RR ..
-            constexpr int PR = 64 / CL, RR = 64 / CR;
-            // (recomputed in every tile: kept, they would cost registers)
-            int l = lane;
-            asm volatile("" : "+v"(l));
-            const auto latent_chunk = [&](int r) {
-                return (unsigned)(
-                    ((l % CL) ^ tile_key<CL>(group * GROUPS * 8 + r)) * 16);
-            };
-            const auto rotary_chunk = [&](int r) {
-                return (unsigned)(R * 2 + ((l % CR)
-                    ^ tile_key<CR>(group * GROUPS * 8 + r)) * 16);
-            };
-            if (a.page_of_groups) {
-                // groups of 8 tokens never straddle a page: their places
-                // are the same for all lanes and live in scalar registers
-                CacheGroup from[GROUPS];
+        // The pieces of a tile that this wave loads: LP of the latent part,
+        // PR rows each, and RP of the rotary part, RR rows each.
+        constexpr int PR = 64 / CL, RR = 64 / CR;
+        constexpr int LP = GROUPS * 8 / PR, RP = (GROUPS * 8 + RR - 1) / RR;
+        // Groups of 8 tokens that never straddle a page have places that are
+        // the same for all lanes and live in scalar registers. For any other
+        // page size lane l has the place of token l, found one tile earlier.
+        CacheGroup from[GROUPS];
+        long place = 0, ahead = GROUPED ? 0 : locate(t0);
+        const auto find = [&](int t) {
+            if constexpr (GROUPED) {
+                const int tok0 = t * KEYS + share * TOKENS
+                                 + group * GROUPS * 8;
                 #pragma unroll
                 for (int g = 0; g < GROUPS; ++g) {
                     // behind the end, the last group once more
@@ -272,52 +266,41 @@ void latent_cache_kernel(CacheArgs a) {
                         + (long)(tok - slot * a.page_size) * a.c_t * 2;
                     from[g].last = len - 1 - tok;
                 }
-                #pragma unroll
-                for (int p = 0; p < GROUPS * 8 / PR; ++p) {
-                    const int r = p * PR + (PR == 1 ? 0 : lane / CL);
-                    const CacheGroup& f = from[p * PR / 8];
-                    if constexpr (PR == 1)
-                        // a row's place is the same for all lanes
-                        tile_load(f.at + (long)(min(r % 8, f.last) * step)
-                                  + latent_chunk(r), image + p * PR * R);
-                    else
-                        tile_load(f.at + (unsigned)(min(r % 8, f.last) * step
-                                                    + latent_chunk(r)),
-                                  image + p * PR * R);
-                }
-                #pragma unroll
-                for (int p = 0; p < (GROUPS * 8 + RR - 1) / RR; ++p) {
-                    const int r = p * RR + lane / CR;
-                    CacheGroup f = from[p * RR / 8];
-                    if (RR == 16 && GROUPS > 1 && lane >= 32)
-                        f = from[(p * RR / 8 + 1) % GROUPS];
-                    if (r < GROUPS * 8)
-                        tile_load(f.at + (unsigned)(min(r % 8, f.last) * step
-                                                    + rotary_chunk(r)),
-                                  rotary + p * RR * DR);
-                }
             } else {
-                // any other page size: lane l has the place of token l, found
-                // one tile earlier and before that tile's pieces
-                const long place = ahead;
+                place = ahead;
                 if (t + 1 < t1) ahead = locate(t + 1);
-                #pragma unroll
-                for (int p = 0; p < GROUPS * 8 / PR; ++p) {
-                    const int r = p * PR + lane / CL;
-                    tile_load(
-                        reinterpret_cast<const char*>(a.cache)
-                        + __shfl(place, r) + latent_chunk(r),
-                        image + p * PR * R);
-                }
-                #pragma unroll
-                for (int p = 0; p < (GROUPS * 8 + RR - 1) / RR; ++p) {
-                    const int r = p * RR + lane / CR;
-                    const long from = __shfl(place, r);
-                    if (r < GROUPS * 8)
-                        tile_load(
-                            reinterpret_cast<const char*>(a.cache) + from
-                            + rotary_chunk(r), rotary + p * RR * DR);
-                }
+            }
+        };
+        const auto load = [&](int p, int buf) {
+            // (recomputed for every piece: kept, they would cost registers)
+            unsigned l = lane;
+            asm volatile("" : "+v"(l));
+            const bool rotary = p >= LP;
+            const int q = rotary ? p - LP : p;
+            const int row0 = q * (rotary ? RR : PR);
+            T* to = images + buf * TILE + (rotary ? TOKENS * R : 0)
+                    + (group * GROUPS * 8 + row0) * (rotary ? DR : R);
+            const int r = row0 + (int)(rotary ? l / CR
+                                              : PR == 1 ? 0 : l / CL);
+            const int key = group * GROUPS * 8 + r;
+            const unsigned chunk = rotary
+                ? R * 2 + ((l % CR) ^ tile_key<CR>(key)) * 16
+                : ((l % CL) ^ tile_key<CL>(key)) * 16;
+            // half a wave loads the rotary part of one group of 32 columns
+            if (rotary && GROUPS * 8 < RR && l >= 32) return;
+            if constexpr (GROUPED) {
+                CacheGroup f = from[row0 / 8];
+                if (rotary && RR == 16 && GROUPS > 1 && l >= 32)
+                    f = from[(row0 / 8 + 1) % GROUPS];
+                if (!rotary && PR == 1)
+                    tile_load(f.at + (long)(min(r % 8, f.last) * step),
+                              chunk, to);
+                else
+                    tile_load(f.at + (unsigned)(min(r % 8, f.last) * step
+                                                + chunk), to);
+            } else {
+                tile_load(reinterpret_cast<const char*>(a.cache)
+                          + __shfl(place, r) + chunk, to);
             }
         };
 
@@ -325,26 +308,41 @@ void latent_cache_kernel(CacheArgs a) {
         float top = -INFINITY, sub = 0.0f, sum = 0.0f;
         // every wave is done with the LDS of the segment before
         __syncthreads();
-        // Turn t loads tile t + LEAD and uses tile t; the first turns only
-        // load. Waves that share tiles load one tile ahead, behind the barrier
-        // that ends its buffer's use; a wave alone loads two ahead, after its
-        // own use of the buffer.
-        constexpr int LEAD = ALONE ? 2 : 1;
-        for (int t = t0 - LEAD; t < t1; ++t) {
+        const auto load_all = [&](int t) {
+            if constexpr (ALONE) find(t);
+            #pragma unroll
+            for (int p = 0; p < PIECES; ++p) load(p, t & (BUFS - 1));
+        };
+        if constexpr (!ALONE)
+            #pragma unroll 1
+            for (int t = t0; t < min(t0 + LEAD, t1); ++t) {
+                find(t);
+                load_all(t);
+            }
+        #pragma unroll
+        for (int i = 0; i < (R + DR) / 32; ++i) tile_settle(bq[i]);
+        // Turn t uses tile t and loads tile t + LEAD; the first turns of a
+        // wave alone only load. LDS-DMA arrives in order, so the pieces of
+        // later tiles may stay on their way.
+        for (int t = ALONE ? t0 - LEAD : t0; t < t1; ++t) {
+            const bool more = t + LEAD < t1;
+            const int later = min(t1 - 1 - t, ALONE ? 1 : LEAD - 1);
+            if (!ALONE || t >= t0) {
+            if (later == 2)
+                asm volatile("s_waitcnt vmcnt(%0)" ::"i"(2 * PIECES)
+                             : "memory");
+            else if (later == 1)
+                asm volatile("s_waitcnt vmcnt(%0)" ::"i"(PIECES) : "memory");
+            else
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            }
             if constexpr (!ALONE) {
-                tile_arrive();
-                if (t + LEAD < t1) stage(t + LEAD, (t + LEAD) & 1);
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+                if (more) find(t + LEAD);
             }
-            if (t >= t0 && live) {
-            if constexpr (ALONE) {
-                // all but the next tile's pieces have arrived
-                if (t + 1 < t1)
-                    asm volatile("s_waitcnt vmcnt(%0)" ::"i"(PIECES)
-                                 : "memory");
-                else
-                    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            }
-            const unsigned image = lds + (t & 1) * TILE * 2;
+            if (live && (!ALONE || t >= t0)) {
+            const unsigned image = lds + (t & (BUFS - 1)) * TILE * 2;
             const unsigned latent = tile_row_base<CL, 16>(image, lane);
             const unsigned rope = tile_row_base<CR, 16>(
                 image + TOKENS * R * 2, lane);
@@ -371,21 +369,29 @@ void latent_cache_kernel(CacheArgs a) {
             static_assert(VF % AHEAD == 0, "whole batches");
             #pragma unroll
             for (int j = 0; j < AHEAD; ++j) f[0][j] = key(j);
+            // A wave that issues a load waits until the ones before it, also
+            // those of other waves, are accepted, about 24 cycles for 1 KiB:
+            // they go out one by one between the batches of both products.
+            constexpr int EACH = (PIECES + KB + VB - 1) / (KB + VB);
+            const auto load_between = [&](int b) {
+                if (!ALONE && more)
+                    #pragma unroll
+                    for (int p = b * EACH; p < (b + 1) * EACH; ++p)
+                        if (p < PIECES) load(p, (t + LEAD) & (BUFS - 1));
+            };
             #pragma unroll
             for (int b = 0; b < KB; ++b) {
-                #pragma unroll
-                for (int j = 0; j < AHEAD; ++j)
-                    if ((b + 1) * AHEAD + j < KF)
-                        f[(b + 1) & 1][j] = key((b + 1) * AHEAD + j);
-                __builtin_amdgcn_sched_barrier(0);
+                load_between(b);
                 #pragma unroll
                 for (int j = 0; j < AHEAD; ++j) {
                     const int k = b * AHEAD + j;
+                    if (k + AHEAD < KF)
+                        f[(b + 1) & 1][j] = key(k + AHEAD);
                     if (k < KF)
                         s[k % SUB] = tile_mfma(f[b & 1][j], bq[k / SUB],
                                                s[k % SUB]);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-                __builtin_amdgcn_sched_barrier(0);
             }
             // the first values, while the weights are formed
             #pragma unroll
@@ -439,21 +445,20 @@ void latent_cache_kernel(CacheArgs a) {
             }
             #pragma unroll
             for (int b = 0; b < VB; ++b) {
-                #pragma unroll
-                for (int j = 0; j < AHEAD; ++j)
-                    if (b + 1 < VB)
-                        f[(b + 1) & 1][j] = val((b + 1) * AHEAD + j);
-                __builtin_amdgcn_sched_barrier(0);
+                load_between(KB + b);
                 #pragma unroll
                 for (int j = 0; j < AHEAD; ++j) {
                     const int k = b * AHEAD + j;
+                    if (b + 1 < VB) f[(b + 1) & 1][j] = val(k + AHEAD);
                     acc[k % NT] = tile_mfma(f[b & 1][j], w[k / NT],
                                             acc[k % NT]);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-                __builtin_amdgcn_sched_barrier(0);
             }
             }
-            if (ALONE && t + LEAD < t1) stage(t + LEAD, t & 1);
+            // a wave alone is done with the buffer only now; one without rows
+            // does its part of the loads
+            if (more && (ALONE || !live)) load_all(t + LEAD);
         }
         sum += __shfl_xor(sum, 16);
         sum += __shfl_xor(sum, 32);
@@ -466,7 +471,7 @@ void latent_cache_kernel(CacheArgs a) {
             constexpr int STEP = 64 * WR;
             float* give = reinterpret_cast<float*>(smem) + group * 64 + lane;
             float* stat = give + STEP * NT * 4;
-            static_assert((NT * 4 + 2) * STEP * 4 <= WT * 2 * TILE * 2,
+            static_assert((NT * 4 + 2) * STEP * 4 <= WT * BUFS * TILE * 2,
                           "the sums must fit in the tiles' LDS");
             if (share == 1) {
                 #pragma unroll
@@ -643,8 +648,14 @@ bool cache_rows_ok(const torch::Tensor& x) {
 
 template <typename T, int R, int DR, int WR, int WT>
 void cache_launch_shape(const CacheArgs& a, int blocks) {
-    hipLaunchKernelGGL((latent_cache_kernel<T, R, DR, WR, WT>), dim3(blocks),
-                       dim3(64 * WR * WT), 0, pe_current_stream(), a);
+    if (a.page_size % 8 == 0)
+        hipLaunchKernelGGL((latent_cache_kernel<T, R, DR, WR, WT, true>),
+                           dim3(blocks), dim3(64 * WR * WT), 0,
+                           pe_current_stream(), a);
+    else
+        hipLaunchKernelGGL((latent_cache_kernel<T, R, DR, WR, WT, false>),
+                           dim3(blocks), dim3(64 * WR * WT), 0,
+                           pe_current_stream(), a);
     hipLaunchKernelGGL((latent_cache_join_kernel<T, R>),
                        dim3((a.rows + 15) / 16, R / 64, a.B), dim3(256), 0,
                        pe_current_stream(), a, a.row_groups * WR);
@@ -747,20 +758,20 @@ torch::Tensor latent_cache_attention_op(
     a.pages = cache.size(0);
     a.page_size = page;
     a.page_shift = (page & (page - 1)) == 0 ? __builtin_ctzl(page) : -1;
-    a.page_of_groups = page % 8 == 0;
     a.B = B, a.H = H, a.Sq = Sq, a.table_width = width;
     a.rows = Sq * H;
     a.scale = scale * 1.4426950408889634;
     const int block_rows = a.rows <= 16 ? 16 : a.rows <= 32 ? 32 : 64;
     a.row_groups = (a.rows + block_rows - 1) / block_rows;
+    a.tile_shift = block_rows == 64 ? 5 : 6;
     // LDS holds one block a CU; no more runs than there can be tiles
-    const int64_t most = B * ((page * width + KEYS - 1) / KEYS);
+    const int64_t most = B * ((page * width >> a.tile_shift) + 1);
     TORCH_CHECK_VALUE(most < (1L << 31) - 512,
                       "latent_cache_attention: too many tokens");
     a.runs = std::min<int64_t>(std::max(256 / a.row_groups, 1), most);
     // measured on one sequence of 8192: 64 rows 32, 30, 29, 31 us for 1 to 4
     // tiles; 16 rows of 517 tokens 13, 17, 17, 21 us
-    a.least = block_rows == 64 ? 2 : 1;
+    a.least = block_rows == 64 ? 4 : 1;
     const int blocks = a.runs * a.row_groups;
     const int64_t slots = (B + a.runs) * a.row_groups;
     auto part = torch::empty({slots * block_rows * (latent_dim + 2)},

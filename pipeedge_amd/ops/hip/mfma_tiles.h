@@ -63,11 +63,47 @@ __device__ __forceinline__ constexpr int tile_key(int row) {
         return low;
 }
 
-// 16 bytes a lane from global memory into LDS at base + lane * 16
+// 16 bytes a lane from global memory into LDS at dst + lane * 16 (LDS-DMA).
+// Written out because the compiler, which cannot tell the buffers of an image
+// apart, would wait for all pieces on their way before each transposing read
+// (an 8192-token prompt with 16 heads: 343 us, 26% of them in such waits). It
+// does not count these loads, which only makes its own waits longer than they
+// need to be; waiting for a piece is the caller's part, with an explicit
+// s_waitcnt vmcnt and a barrier, whose clobbers also keep LDS accesses on
+// their side. The load has no output register that could be reused early.
 __device__ __forceinline__ void tile_load(const void* src, void* dst) {
-    __builtin_amdgcn_global_load_lds(
-        (const __attribute__((address_space(1))) unsigned int*)src,
-        (__attribute__((address_space(3))) unsigned int*)dst, 16, 0, 0);
+    // dst is the same for all lanes, which the compiler may have lost
+    const int to = __builtin_amdgcn_readfirstlane(
+        (int)reinterpret_cast<uintptr_t>(dst));
+    asm volatile("s_mov_b32 m0, %0\n\t"
+                 "s_nop 0\n\t"
+                 "global_load_lds_dwordx4 %1, off"
+                 :
+                 : "s"(to), "v"(src)
+                 : "m0");
+}
+// the same from base + offset, base the same for all lanes
+__device__ __forceinline__ void tile_load(const void* base, unsigned offset,
+                                          void* dst) {
+    const int to = __builtin_amdgcn_readfirstlane(
+        (int)reinterpret_cast<uintptr_t>(dst));
+    const uintptr_t b = reinterpret_cast<uintptr_t>(base);
+    const uintptr_t from =
+        (uintptr_t)(unsigned)__builtin_amdgcn_readfirstlane((int)b)
+        | (uintptr_t)__builtin_amdgcn_readfirstlane((int)(b >> 32)) << 32;
+    asm volatile("s_mov_b32 m0, %0\n\t"
+                 "s_nop 0\n\t"
+                 "global_load_lds_dwordx4 %1, %2"
+                 :
+                 : "s"(to), "v"(offset), "s"(from)
+                 : "m0");
+}
+
+// Makes the compiler wait for a loaded value here: at its first use inside a
+// loop it would wait in every turn, and for the pieces on their way as well.
+template <typename V>
+__device__ __forceinline__ void tile_settle(V& v) {
+    asm volatile("" : "+v"(v));
 }
 
 // Wait for this wave's LDS-DMA, then for all waves. The clobbers keep LDS
