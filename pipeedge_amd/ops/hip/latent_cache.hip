@@ -21,11 +21,13 @@
 // second operand as they are. One LDS image of a tile serves both products,
 // read by rows for the scores and by columns, through the transposing reads,
 // for the values. The accumulators take R / 4 registers and the query
-// operands (R + DR) / 8, so two waves share a SIMD: 8 waves of one block, 128
-// rows, use a tile of 64 tokens together. With fewer rows the waves also
-// split a tile's tokens, 32 each, and join their sums at the segment's end;
-// up to 16 rows a wave loads its own tokens, two tiles ahead, and waits for
-// nobody else.
+// operands (R + DR) / 8. A block has up to 64 rows, one or two waves a SIMD,
+// and its waves share the tokens of a tile; where two waves have the same
+// rows, they take 32 tokens of a tile each and join their sums at the
+// segment's end. Up to 16 rows a wave loads its own tokens, two tiles ahead,
+// and waits for nobody else. 16 heads are bound by memory (64 ragged sequences
+// up to 4096, 165 MB: 35 us, 4.7 TB/s, and 5 us to join), 128 heads by the
+// instructions around the MFMAs, which keep them busy a third of the time.
 #include <torch/extension.h>
 
 #include <c10/core/DeviceGuard.h>
@@ -469,37 +471,40 @@ void latent_cache_kernel(CacheArgs a) {
             // the second wave of a group hands its sums to the first; the
             // barrier above ended all use of the tiles
             constexpr int STEP = 64 * WR;
-            float* give = reinterpret_cast<float*>(smem) + group * 64 + lane;
-            float* stat = give + STEP * NT * 4;
-            static_assert((NT * 4 + 2) * STEP * 4 <= WT * BUFS * TILE * 2,
+            f32x4* give = reinterpret_cast<f32x4*>(smem) + group * 64 + lane;
+            float2* stat = reinterpret_cast<float2*>(
+                reinterpret_cast<f32x4*>(smem) + NT * STEP)
+                + group * 64 + lane;
+            static_assert(NT * STEP * 16 + STEP * 8 <= WT * BUFS * TILE * 2,
                           "the sums must fit in the tiles' LDS");
             if (share == 1) {
                 #pragma unroll
-                for (int n = 0; n < NT; ++n)
-                    #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        give[(n * 4 + i) * STEP] = acc[n][i];
-                stat[0] = top;
-                stat[STEP] = sum;
+                for (int n = 0; n < NT; ++n) give[n * STEP] = acc[n];
+                *stat = make_float2(top, sum);
             }
             __syncthreads();
             if (share == 0) {
-                const float top2 = stat[0], sum2 = stat[STEP];
-                const float next = fmaxf(top, top2);
+                const float2 other = *stat;
+                const float next = fmaxf(top, other.x);
                 // a share that saw no token has nothing to give
                 const float f1 = top == -INFINITY
                     ? 0.0f : __builtin_amdgcn_exp2f(top - next);
-                const float f2 = top2 == -INFINITY
-                    ? 0.0f : __builtin_amdgcn_exp2f(top2 - next);
+                const float f2 = other.x == -INFINITY
+                    ? 0.0f : __builtin_amdgcn_exp2f(other.x - next);
                 top = next;
                 sum = (sum == sum ? sum * f1 : sum)
-                      + (sum2 == sum2 ? sum2 * f2 : sum2);
+                      + (other.y == other.y ? other.y * f2 : other.y);
                 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+                for (int n = 0; n < NT; n += 4) {
+                    f32x4 taken[4];
                     #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        acc[n][i] = acc[n][i] * f1
-                                    + give[(n * 4 + i) * STEP] * f2;
+                    for (int j = 0; j < 4; ++j)
+                        taken[j] = give[(n + j) * STEP];
+                    __builtin_amdgcn_sched_barrier(0);
+                    #pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        acc[n + j] = acc[n + j] * f1 + taken[j] * f2;
+                }
             }
         }
 
@@ -663,7 +668,10 @@ void cache_launch_shape(const CacheArgs& a, int blocks) {
 
 template <typename T, int R, int DR>
 void cache_launch(const CacheArgs& a, int block_rows, int blocks) {
-    if (block_rows == 64) cache_launch_shape<T, R, DR, 4, 1>(a, blocks);
+    if (block_rows == 64 && a.tile_shift == 6)
+        cache_launch_shape<T, R, DR, 4, 2>(a, blocks);
+    else if (block_rows == 64)
+        cache_launch_shape<T, R, DR, 4, 1>(a, blocks);
     else if (block_rows == 32) cache_launch_shape<T, R, DR, 2, 2>(a, blocks);
     else cache_launch_shape<T, R, DR, 1, 2>(a, blocks);
 }
@@ -763,15 +771,20 @@ torch::Tensor latent_cache_attention_op(
     a.scale = scale * 1.4426950408889634;
     const int block_rows = a.rows <= 16 ? 16 : a.rows <= 32 ? 32 : 64;
     a.row_groups = (a.rows + block_rows - 1) / block_rows;
-    a.tile_shift = block_rows == 64 ? 5 : 6;
     // LDS holds one block a CU; no more runs than there can be tiles
-    const int64_t most = B * ((page * width >> a.tile_shift) + 1);
-    TORCH_CHECK_VALUE(most < (1L << 31) - 512,
+    const int64_t most = B * ((page * width + 63) / 64);
+    TORCH_CHECK_VALUE(most < (1L << 30),
                       "latent_cache_attention: too many tokens");
     a.runs = std::min<int64_t>(std::max(256 / a.row_groups, 1), most);
-    // measured on one sequence of 8192: 64 rows 32, 30, 29, 31 us for 1 to 4
-    // tiles; 16 rows of 517 tokens 13, 17, 17, 21 us
-    a.least = block_rows == 64 ? 4 : 1;
+    // 64 rows: two waves on a SIMD, each with half of a tile, hide more of
+    // each other's latencies, but have to join at a segment's end. By the most
+    // tokens that a run can have, us with one wave and with two: 2048 (32
+    // tiles) 115 and 101, 1024 67 and 67, 512 47 and 52.
+    const bool halves = block_rows < 64 || most >= 16 * a.runs;
+    a.tile_shift = halves ? 6 : 5;
+    // measured on one sequence of 8192: 64 rows 32, 30, 29, 31 us for runs of
+    // 64 to 256 tokens; 16 rows of 517 tokens 13, 17, 17, 21 us
+    a.least = block_rows < 64 ? 1 : halves ? 2 : 4;
     const int blocks = a.runs * a.row_groups;
     const int64_t slots = (B + a.runs) * a.row_groups;
     auto part = torch::empty({slots * block_rows * (latent_dim + 2)},
