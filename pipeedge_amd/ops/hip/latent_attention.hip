@@ -86,28 +86,46 @@ __global__ __launch_bounds__(256, 2) void latent_attention_kernel(
 
     const T* kv = reinterpret_cast<const T*>(a.kv) + b * a.kv_b + h * a.kv_h;
     const T* kr = reinterpret_cast<const T*>(a.k_rope) + b * a.r_b;
-    // Tokens behind the last one are read as the last one: their weights
-    // are zero, and what lies in the padding cannot reach the sums.
+    // A piece's place in its tile: the lane's row and chunk, as a byte offset
+    // from the tile's first token. Tokens behind the last one are read as the
+    // last one: their weights are zero, and what lies in the padding cannot
+    // reach the sums. That only changes the last tile's offsets.
+    constexpr int NP = CN / 4, RP = CR / 4;
+    unsigned kv_at[NP], r_at[RP];
+    const auto place = [&](int last) {
+        #pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            const int r = (wid + 4 * i) * (64 / CN) + lane / CN;
+            const int c = (lane % CN) ^ tile_key<CN>(r);
+            kv_at[i] = (unsigned)(min(r, last) * (int)a.kv_s + c * 8) * 2;
+        }
+        #pragma unroll
+        for (int i = 0; i < RP; ++i) {
+            const int r = (wid + 4 * i) * (64 / CR) + lane / CR;
+            const int c = (lane % CR) ^ tile_key<CR>(r);
+            r_at[i] = (unsigned)(min(r, last) * (int)a.r_s + c * 8) * 2;
+        }
+    };
+    place(KEYS);
     const auto stage = [&](int t, int buf) {
         T* base = smem + buf * TILE;
         const int tok0 = t * KEYS;
+        if (tok0 + KEYS > len) {
+            tile_rare();
+            place(len - 1 - tok0);
+        }
+        const T* k0 = kv + tok0 * a.kv_s;
+        const T* r0 = kr + tok0 * a.r_s;
         #pragma unroll
-        for (int i = 0; i < CN / 4; ++i) {
+        for (int i = 0; i < NP; ++i) {
             const int p = wid + 4 * i;
-            const int r = p * (64 / CN) + lane / CN;
-            const int c = (lane % CN) ^ tile_key<CN>(r);
-            const T* src = kv + min(tok0 + r, len - 1) * a.kv_s + c * 8;
-            tile_load(src, base + p * 512);
-            tile_load(src + DN, base + KEYS * (DN + DR) + p * 512);
+            tile_load(k0, kv_at[i], base + p * 512);
+            tile_load(k0 + DN, kv_at[i], base + KEYS * (DN + DR) + p * 512);
         }
         #pragma unroll
-        for (int i = 0; i < CR / 4; ++i) {
-            const int p = wid + 4 * i;
-            const int r = p * (64 / CR) + lane / CR;
-            const int c = (lane % CR) ^ tile_key<CR>(r);
-            tile_load(kr + min(tok0 + r, len - 1) * a.r_s + c * 8,
-                            base + KEYS * DN + p * 512);
-        }
+        for (int i = 0; i < RP; ++i)
+            tile_load(r0, r_at[i],
+                      base + KEYS * DN + (wid + 4 * i) * 512);
     };
 
     f32x16 acc[NT] = {};
@@ -137,15 +155,16 @@ __global__ __launch_bounds__(256, 2) void latent_attention_kernel(
             #pragma unroll
             for (int m = 0; m < 2; ++m)
                 s[m] = tile_mfma(tile_row_read<T, CN, 32>(nope, m * 32, i),
-                                   bq[i], s[m]);
+                                 bq[i], s[m]);
         #pragma unroll
         for (int i = 0; i < DR / 16; ++i)
             #pragma unroll
             for (int m = 0; m < 2; ++m)
                 s[m] = tile_mfma(tile_row_read<T, CR, 32>(rope, m * 32, i),
-                                   bq[DN / 16 + i], s[m]);
+                                 bq[DN / 16 + i], s[m]);
 
         if (__any(limit < tok0 + KEYS - 1)) {
+            tile_rare();
             #pragma unroll
             for (int m = 0; m < 2; ++m)
                 #pragma unroll
@@ -161,6 +180,7 @@ __global__ __launch_bounds__(256, 2) void latent_attention_kernel(
             for (int i = 0; i < 16; ++i) peak = fmaxf(peak, s[m][i]);
         peak = fmaxf(peak, __shfl_xor(peak, 32)) * a.scale;
         if (__any(peak > top + softmax::SLACK)) {
+            tile_rare();
             const float next = fmaxf(top, peak);
             const float turn = top == -INFINITY
                 ? 0.0f : __builtin_amdgcn_exp2f(top - next);
@@ -294,6 +314,9 @@ torch::Tensor latent_attention_op(
     if (Sk == 0) return out.zero_();
     TORCH_CHECK_VALUE(Sq < (1L << 30) && Sk < (1L << 30),
                       "latent_attention: too many tokens");
+    TORCH_CHECK_VALUE(kv.stride(1) < (1L << 24) &&
+                      k_rope.stride(1) < (1L << 24),
+                      "latent_attention: tokens more than 32 MiB apart");
     const int64_t row_blocks = (Sq + ROWS - 1) / ROWS;
     TORCH_CHECK_VALUE(B * H * row_blocks < (1L << 31),
                       "latent_attention: too many rows");

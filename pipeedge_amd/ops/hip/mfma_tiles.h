@@ -66,11 +66,12 @@ __device__ __forceinline__ constexpr int tile_key(int row) {
 // 16 bytes a lane from global memory into LDS at dst + lane * 16 (LDS-DMA).
 // Written out because the compiler, which cannot tell the buffers of an image
 // apart, would wait for all pieces on their way before each transposing read
-// (an 8192-token prompt with 16 heads: 343 us, 26% of them in such waits). It
-// does not count these loads, which only makes its own waits longer than they
-// need to be; waiting for a piece is the caller's part, with an explicit
-// s_waitcnt vmcnt and a barrier, whose clobbers also keep LDS accesses on
-// their side. The load has no output register that could be reused early.
+// (with tiles of 32 tokens, three ahead, which that had ruled out, 64 ragged
+// cached sequences of 16 heads went from 46 to 41 us). It does not count these
+// loads, which only makes its own waits longer than they need to be; waiting
+// for a piece is the caller's part, with an explicit s_waitcnt vmcnt and a
+// barrier, whose clobbers also keep LDS accesses on their side. The load has
+// no output register that could be reused early.
 __device__ __forceinline__ void tile_load(const void* src, void* dst) {
     // dst is the same for all lanes, which the compiler may have lost
     const int to = __builtin_amdgcn_readfirstlane(
@@ -105,6 +106,10 @@ template <typename V>
 __device__ __forceinline__ void tile_settle(V& v) {
     asm volatile("" : "+v"(v));
 }
+
+// At the head of a rare branch: without it the compiler computes the branch's
+// values in every turn and selects, which costs more than the branch.
+__device__ __forceinline__ void tile_rare() { asm volatile(""); }
 
 // Wait for this wave's LDS-DMA, then for all waves. The clobbers keep LDS
 // accesses on their side of the barrier.
