@@ -8,10 +8,18 @@
 // value columns as the rows, queries as the columns of 32x32x16 MFMAs), so a
 // lane holds scores of one query only: softmax needs one exchange between
 // the halves of a wave, and the weights are the second product's operand as
-// they are, without leaving their lane. Tiles go to LDS by LDS-DMA while the previous one is used;
-// the shared rotary key is staged as it is and never copied per head.
-// Bound by the matrix cores and the LDS reads that feed them.
+// they are, without leaving their lane. Tiles go to LDS by LDS-DMA while the
+// previous one is used; the shared rotary key is staged as it is and never
+// copied per head.
+//
+// Bound by what a wave does in turn: 40 MFMAs a tile (1280 cycles of a SIMD),
+// then 32 exponentials a lane and their sums, with a second wave on the SIMD
+// to fill the gaps. 4099 queries against 8198 keys, 16 heads of 128 + 64, bf16
+// causal: 318 us, 810 TFLOP/s of about 1450 that a large matrix product
+// reaches; without exponentials 7% less, without loads 17% less time.
 #include <torch/extension.h>
+
+#include <algorithm>
 
 #include <c10/core/DeviceGuard.h>
 
@@ -24,10 +32,12 @@ struct LatentArgs {
     const void* kv;
     const void* k_rope;
     void* out;                  // [B, Sq, H, DN]
+    float* sums;                // [parts, B, Sq, H, DN], for parts > 1
+    float2* stats;              // [parts, B, Sq, H]: top and total
     const int* lengths;         // [B] or nullptr: all keys
     const int* past;            // [B] or nullptr: Sk - Sq
     long q_b, q_s, q_h, kv_b, kv_s, kv_h, r_b, r_s;   // strides in elements
-    int B, H, Sq, Sk, row_blocks;
+    int B, H, Sq, Sk, row_blocks, parts;
     bool causal;
     float scale;                // times log2(e)
 };
@@ -46,12 +56,16 @@ __global__ __launch_bounds__(256, 2) void latent_attention_kernel(
     constexpr int TILE = KEYS * (2 * DN + DR);
     __shared__ __attribute__((aligned(256))) T smem[2 * TILE];
 
-    const int id = xcd_contiguous(blockIdx.x, gridDim.x);
-    const int bh = id / a.row_blocks;
+    // The last rows of all heads first: causal blocks see more keys the later
+    // they are, and what starts last should be short (8192 tokens, 12 heads:
+    // 320 us with head after head, 254 so). Blocks go to the 8 XCDs in turn,
+    // so the blocks of a head, which read the same keys, also share an L2 if
+    // the number of heads is a multiple of 8, as it mostly is.
+    const int heads = a.B * a.H;
+    const int rest = blockIdx.x / heads, bh = blockIdx.x - rest * heads;
+    const int back = rest / a.parts, part = rest - back * a.parts;
     const int b = bh / a.H, h = bh - b * a.H;
-    int rb = id - bh * a.row_blocks;
-    rb = a.row_blocks - 1 - rb;
-    const int q0 = rb * ROWS;
+    const int q0 = (a.row_blocks - 1 - back) * ROWS;
 
     const int tid = threadIdx.x;
     const int lane = tid & 63, l31 = lane & 31, hi = lane >> 5;
@@ -132,10 +146,12 @@ __global__ __launch_bounds__(256, 2) void latent_attention_kernel(
     float top = -INFINITY, sub = 0.0f, total = 0.0f;
 
     const unsigned lds = tile_lds(smem);
-    if (tiles > 0) stage(0, 0);
+    const int first = (long)tiles * part / a.parts;
+    const int end = (long)tiles * (part + 1) / a.parts;
+    if (first < end) stage(first, first & 1);
     #pragma unroll
     for (int i = 0; i < (DN + DR) / 16; ++i) tile_settle(bq[i]);
-    for (int t = 0; t < tiles; ++t) {
+    for (int t = first; t < end; ++t) {
         const unsigned image = lds + (t & 1) * TILE * 2;
         const unsigned nope = tile_row_base<CN, 32>(image, lane);
         const unsigned rope =
@@ -145,7 +161,7 @@ __global__ __launch_bounds__(256, 2) void latent_attention_kernel(
         // this wave's part of tile t has arrived; behind the barrier all
         // parts have, and every wave is done with the other buffer
         tile_arrive();
-        if (t + 1 < tiles) stage(t + 1, (t + 1) & 1);
+        if (t + 1 < end) stage(t + 1, (t + 1) & 1);
         const int tok0 = t * KEYS;
         if (tok0 > wave_last) continue;
 
@@ -216,6 +232,23 @@ __global__ __launch_bounds__(256, 2) void latent_attention_kernel(
     }
 
     total += __shfl_xor(total, 32);
+    if (a.parts > 1) {
+        if (row >= a.Sq) return;
+        const long at = (((long)part * a.B + b) * a.Sq + row) * a.H + h;
+        if (hi == 0) a.stats[at] = make_float2(top, total);
+        if (total == 0.0f) return;      // not read either
+        float* sums = a.sums + at * DN + hi * 4;
+        #pragma unroll
+        for (int n = 0; n < NT; ++n)
+            #pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                f32x4 o;
+                #pragma unroll
+                for (int j = 0; j < 4; ++j) o[j] = acc[n][g * 4 + j];
+                *reinterpret_cast<f32x4*>(sums + n * 32 + g * 8) = o;
+            }
+        return;
+    }
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
     if (row < a.Sq) {
         T* out = reinterpret_cast<T*>(a.out)
@@ -234,6 +267,35 @@ __global__ __launch_bounds__(256, 2) void latent_attention_kernel(
     }
 }
 
+// Joins the parts of each row, in their order: DN / 4 lanes a row.
+template <typename T, int DN>
+__global__ __launch_bounds__(256) void latent_join_kernel(
+        const float* __restrict__ sums, const float2* __restrict__ stats,
+        T* __restrict__ out, long rows, int parts) {
+    constexpr int LANES = DN / 4;
+    const long row = (long)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+    if (row >= rows) return;
+    const int col = threadIdx.x % LANES * 4;
+    float top = -INFINITY;
+    for (int p = 0; p < parts; ++p) top = fmaxf(top, stats[p * rows + row].x);
+    float total = 0.0f;
+    f32x4 sum = {};
+    #pragma unroll 4
+    for (int p = 0; p < parts; ++p) {
+        const float2 s = stats[p * rows + row];
+        if (s.y == 0.0f) continue;
+        const float w = __builtin_amdgcn_exp2f(s.x - top);
+        total += s.y * w;
+        sum += *reinterpret_cast<const f32x4*>(
+            sums + (p * rows + row) * DN + col) * w;
+    }
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    typename TileVec<T>::v4 o;
+    #pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] = (T)(sum[j] * inv);
+    *reinterpret_cast<typename TileVec<T>::v4*>(out + row * DN + col) = o;
+}
+
 // 16-byte accesses need strides and addresses of 8 elements
 torch::Tensor latent_aligned(const torch::Tensor& x) {
     bool ok = reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0 &&
@@ -247,6 +309,13 @@ template <typename T, int DN, int DR>
 void latent_launch(const LatentArgs& a, long blocks) {
     hipLaunchKernelGGL((latent_attention_kernel<T, DN, DR>), dim3(blocks),
                        dim3(256), 0, pe_current_stream(), a);
+    if (a.parts == 1) return;
+    const long rows = (long)a.B * a.Sq * a.H;
+    const int block_rows = 256 / (DN / 4);
+    hipLaunchKernelGGL((latent_join_kernel<T, DN>),
+                       dim3((rows + block_rows - 1) / block_rows), dim3(256),
+                       0, pe_current_stream(), a.sums, a.stats,
+                       reinterpret_cast<T*>(a.out), rows, a.parts);
 }
 
 template <typename T>
@@ -340,12 +409,31 @@ torch::Tensor latent_attention_op(
     a.kv_b = kva.stride(0), a.kv_s = kva.stride(1), a.kv_h = kva.stride(2);
     a.r_b = ra.stride(0), a.r_s = ra.stride(1);
     a.B = B, a.H = H, a.Sq = Sq, a.Sk = Sk, a.row_blocks = row_blocks;
+    // Few blocks split the keys and a second kernel joins the parts: two
+    // blocks a CU, one if all have the same work (256 blocks of 2048 tokens:
+    // 57 us in one part, 62 in two; causal 54 and 50). A part has 8 tiles or
+    // more, with a few rows, whose sums are cheap to pass on, 4 (us in one
+    // part, with 4 and with 8 tiles a part; 16 heads: 64 rows of 8192 tokens
+    // 176, 45, 34; 1 row of 517: 20, 17, 20; 4096 tokens, 4 heads: 92 to 50).
+    int64_t blocks = B * H * row_blocks;
+    const int64_t tiles = (Sk + KEYS - 1) / KEYS;
+    a.parts = std::max<int64_t>(1, std::min((causal ? 512 : 256) / blocks,
+                                            tiles / (Sq <= 32 ? 4 : 8)));
+    torch::Tensor sums, stats;
+    if (a.parts > 1) {
+        blocks *= a.parts;
+        const auto f32 = q.options().dtype(torch::kFloat);
+        sums = torch::empty({a.parts, B, Sq, H, nope}, f32);
+        stats = torch::empty({a.parts, B, Sq, H, 2}, f32);
+        a.sums = sums.data_ptr<float>();
+        a.stats = reinterpret_cast<float2*>(stats.data_ptr<float>());
+    }
     a.causal = causal;
     a.scale = scale * 1.4426950408889634;
     if (dtype == torch::kBFloat16)
-        latent_dispatch<__bf16>(a, nope, rope, B * H * row_blocks);
+        latent_dispatch<__bf16>(a, nope, rope, blocks);
     else
-        latent_dispatch<_Float16>(a, nope, rope, B * H * row_blocks);
+        latent_dispatch<_Float16>(a, nope, rope, blocks);
     HIP_CHECK_LAST();
     return out;
 }

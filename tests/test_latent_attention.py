@@ -119,6 +119,38 @@ def test_expanded_padding(device, causal, sq, sk, lengths, past):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("sq,sk,h,nope,rope,lengths,past", [
+    (1, 512, 1, 64, 32, None, None),
+    (1, 1500, 3, 128, 64, [1500, 1, 0, 65, 1499], [1499, 0, 0, 64, 0]),
+    (5, 2049, 2, 64, 64, [2049, 4, 600, 0, 1030], [2044, 0, 595, 0, -3]),
+    (40, 1100, 2, 128, 32, [1100, 30, 70, 1025, 512], [1060, 0, 60, 990, 0]),
+    (300, 1061, 1, 128, 64, [1061, 299, 64, 700, 3], [761, 0, 0, 400, 0]),
+])
+def test_expanded_long_keys(device, dtype, causal, sq, sk, h, nope, rope,
+                            lengths, past):
+    """Few queries of many keys, whose range is shared out: sequences that
+    end before most of the shares begin, rows that see a part of one, shares
+    of one tile and of none."""
+    b = 1 if lengths is None else len(lengths)
+    q, kv, k_rope = make_expanded(b, sq, sk, h, nope, rope, dtype, device)
+    n = p = None
+    if lengths is not None:
+        n = torch.tensor(lengths, dtype=torch.int32)
+        p = torch.tensor(past, dtype=torch.int32)
+        for i, end in enumerate(lengths):
+            kv[i, end:] = math.nan
+            k_rope[i, end:] = math.inf
+    out = ops.latent_attention(
+        q, kv, k_rope, causal=causal,
+        lengths=None if n is None else n.to(device),
+        past=None if p is None else p.to(device))
+    check(out, *expanded_exact(q, kv, k_rope, (nope + rope) ** -0.5, causal,
+                               n, p), dtype)
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_expanded_strides(device):
     """Views: heads first, part of wider rows, misaligned storage."""
     dtype = torch.float16
@@ -224,6 +256,34 @@ def test_expanded_graph():
         torch.cuda.synchronize()
         want = ops.latent_attention(q, kv, k_rope, causal=True, lengths=n)
         assert torch.equal(out, want)
+
+
+@pytest.mark.gpu
+def test_expanded_shared_range_graphs():
+    """The partial sums are a graph's own: two graphs and eager calls on
+    another stream, in turn and at once."""
+    many = [make_expanded(3, 4, 1200, 4, 128, 64, torch.bfloat16, "cuda",
+                          seed=i) for i in range(3)]
+    want = [ops.latent_attention(*x, causal=True) for x in many]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for x in many[:2]:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(ops.latent_attention(*x, causal=True))
+    other = torch.cuda.Stream()
+    for _ in range(4):
+        for out in outs:
+            out.zero_()
+        torch.cuda.synchronize()
+        graphs[0].replay()
+        with torch.cuda.stream(other):
+            graphs[1].replay()
+            eager = ops.latent_attention(*many[2], causal=True)
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want[0])
+        assert torch.equal(outs[1], want[1])
+        assert torch.equal(eager, want[2])
 
 
 # ---------------------------------------------------------------- absorbed
