@@ -59,9 +59,9 @@ __device__ __forceinline__ bf16x8 inner_load(const __bf16* p, int k, int K,
 // scaled complementary error function, falls slowly, and a polynomial of
 // degree 8 in 1 / (1 + 0.29 z) follows it to 4e-7 of its value on [0, 16]
 // (own least squares fit, reweighted towards the largest error), where the
-// exponential ends. Half the instructions of the library's erf: with one block
-// a CU nothing else hides the epilogue (64 images of 1280 to 5120 columns:
-// gelu costs 22 us instead of 55).
+// exponential ends. With one block a CU nothing else hides the epilogue (12608
+// rows, 1280 to 5120 columns, rank 64: 239 us without an activation, 251 with
+// this one, 299 with the library's erfc).
 __device__ __forceinline__ float gelu_tail(float x) {
     const float z = fabsf(x);
     const float t = __builtin_amdgcn_rcpf(fmaf(0.29f, z, 1.0f));
@@ -670,33 +670,39 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void adapter_product_kernel(
         }
         const int next = buf + 1 == BUFS ? 0 : buf + 1;
         if (adapter >= 0) stage_adapter(adapter, k, next);
+        // Other requests' rows take nothing, not even the NaN of their own
+        // values times this adapter's, so they keep their sums. That is one
+        // selection a slice: one a step costs more than the products.
+        // Other requests' rows take nothing, not even the NaN of their own
+        // values times this adapter's: they keep their sums. Selected once a
+        // slice, not after each step (12608 rows, 1280 to 5120 columns, rank
+        // 64: 281 us by steps, 275 so; with the operands of all steps in
+        // registers they no longer fit, 358).
+        const int steps = min(STEPS, (a.ad.rank - k0 + 15) / 16);
+        const unsigned from = base + buf * SLICE * 2;
         #pragma unroll
-        for (int step = 0; step < STEPS; ++step) {
-            if (k0 + step * 16 >= a.ad.rank) break;
-            read(buf, step, 0);
-            if (k0 + step * 16 + hi * 8 >= a.ad.rank)
-                #pragma unroll
-                for (int n = 0; n < NI; ++n) fw[0][n] = v8{};
+        for (int m = 0; m < MI; ++m) {
+            if (!__any(id[m] == cur)) continue;
+            f32x16 sum[NI];
             #pragma unroll
-            for (int m = 0; m < MI; ++m) {
-                if (!__any(id[m] == cur)) continue;
-                if (__all(id[m] == cur)) {
-                    #pragma unroll
-                    for (int n = 0; n < NI; ++n)
-                        acc[n][m] = tile_mfma(fw[0][n], fx[0][m], acc[n][m]);
-                    continue;
-                }
-                // other requests' rows take nothing, not even the NaN of
-                // their own values times this adapter's
+            for (int n = 0; n < NI; ++n) sum[n] = acc[n][m];
+            #pragma unroll 1
+            for (int step = 0; step < steps; ++step) {
+                const v8 in = tile_row_read<__bf16, CH, 32>(
+                    from + (BN + wm * MI * 32) * BK * 2, m * 32, step);
                 #pragma unroll
                 for (int n = 0; n < NI; ++n) {
-                    const f32x16 part =
-                        tile_mfma(fw[0][n], fx[0][m], f32x16{});
-                    #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        acc[n][m][i] += id[m] == cur ? part[i] : 0.0f;
+                    v8 up = tile_row_read<__bf16, CH, 32>(
+                        from + wn * NI * 32 * BK * 2, n * 32, step);
+                    if (k0 + step * 16 + hi * 8 >= a.ad.rank) up = v8{};
+                    sum[n] = tile_mfma(up, in, sum[n]);
                 }
             }
+            #pragma unroll
+            for (int n = 0; n < NI; ++n)
+                #pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    acc[n][m][i] = id[m] == cur ? sum[n][i] : acc[n][m][i];
         }
         buf = next;
     }
@@ -926,7 +932,9 @@ torch::Tensor adapter_linear_op(
     const auto x2d = adapter_dense(x.reshape({M, K}));
     const auto w = adapter_dense(weight);
     const auto down_c = adapter_dense(down);
-    // the products of many rows read up 8 of the rank at a time
+    // The products of many rows read up 8 of the rank at a time. Ranks between
+    // are padded here: loads of single elements in each block cost more
+    // (12608 rows, 1280 to 5120, rank 60: 253 us padded, 318 so; 1576 rows, rank 4: 26, 27).
     const bool pad_up = M > STEP_ROWS && r % 8 != 0;
     const auto up_c = pad_up ? at::constant_pad_nd(up, {0, 8 - r % 8})
                              : adapter_dense(up);

@@ -98,6 +98,24 @@ def test_adapter_matches_exact(device, shape, k, n, rank, count):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("shape,k,n,rank,count", [
+    ((11, 197), 72, 3200, 12, 3),
+    ((17, 197), 64, 3100, 3, 4),
+    ((8, 200), 128, 4100, 70, 3),
+    ((3, 100), 64, 300, 1, 5),
+    ((2, 90), 136, 70, 255, 2),
+])
+def test_adapter_odd_ranks(device, shape, k, n, rank, count):
+    x, w, down, up = make(shape, k, n, rank, count, device)
+    ids = (torch.arange(shape[0]) % (count + 1) - 1).int().to(device)
+    args = (x, w, down, up, ids)
+    check(ops.adapter_linear(*args), *args)
+    ids = (torch.arange(shape[0] * shape[1]) * 5 % (count + 2) - 1).int()
+    args = (x, w, down, up, ids.reshape(shape).to(device))
+    check(ops.adapter_linear(*args, act="gelu"), *args, act="gelu")
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_adapter_ids_outside(device):
     """Rows without an adapter get the plain projection, bit for bit."""
     x, w, down, up = make((6, 21), 128, 192, 16, 2, device)
