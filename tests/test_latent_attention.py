@@ -259,6 +259,21 @@ def test_expanded_graph():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("sq,sk", [(100, 100), (3, 1100)])
+def test_expanded_far_sequences(sq, sk):
+    """Sequences more than 2^32 bytes apart."""
+    q, kv, k_rope = make_expanded(2, sq, sk, 2, 128, 64, torch.float16,
+                                  "cuda")
+    want = ops.latent_attention(q, kv, k_rope, causal=True)
+    room = torch.empty(2 ** 31 + 2 * kv[0].numel(), dtype=torch.float16,
+                       device="cuda")
+    far = room.as_strided(kv.shape, (2 ** 31 + 8,) + kv.stride()[1:])
+    far.copy_(kv)
+    assert torch.equal(ops.latent_attention(q, far, k_rope, causal=True),
+                       want)
+
+
+@pytest.mark.gpu
 def test_expanded_shared_range_graphs():
     """The partial sums are a graph's own: two graphs and eager calls on
     another stream, in turn and at once."""
@@ -368,6 +383,40 @@ def test_cache_long_and_many(device):
                                      scale=0.07)
     check(out, *cache_exact(q, cache, table, lengths, 256, 0.07),
           torch.bfloat16)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("h,page", [(16, 64), (32, 5), (70, 16)])
+def test_cache_many_and_one_long(device, h, page):
+    """Runs that hold many short sequences, end in a long one, are inside it
+    and begin with its end."""
+    lengths = [1 + i % 5 for i in range(90)] + [3001] + [i % 3
+                                                         for i in range(80)]
+    q, cache, table, n = make_cache(lengths, 1, h, 256, 64, page,
+                                    torch.float16, device)
+    out = ops.latent_cache_attention(q, cache, table, n, latent_dim=256,
+                                     scale=0.06)
+    check(out, *cache_exact(q, cache, table, lengths, 256, 0.06),
+          torch.float16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("page", [64, 7])
+def test_cache_far_pages(page):
+    """Pages behind 2^32 bytes of a cache are those of a small one."""
+    lengths = [3 * page, 2 * page + 1, 1, 0]
+    q, cache, table, n = make_cache(lengths, 2, 16, 512, 64, page,
+                                    torch.bfloat16, "cuda")
+    want = ops.latent_cache_attention(q, cache, table, n, latent_dim=512,
+                                      scale=0.05)
+    first = 2 ** 32 // (page * 576 * 2) + 1
+    large = torch.empty(first + cache.shape[0], page, 576,
+                        dtype=torch.bfloat16, device="cuda")
+    large[first:] = cache
+    out = ops.latent_cache_attention(
+        q, large, torch.where(table >= 0, table + first, table), n,
+        latent_dim=512, scale=0.05)
+    assert torch.equal(out, want)
 
 
 @pytest.mark.parametrize("device", DEVICES)
