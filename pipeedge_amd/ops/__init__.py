@@ -261,7 +261,8 @@ def latent_attention(q: Tensor, kv: Tensor, k_rope: Tensor, *,
     [B, Sk, H, 2 DN] the keys' plain columns and the values of each head (the
     latent vectors' up-projection, as ``linear`` writes it) and ``k_rope``
     [B, Sk, DR] the rotated key columns that all heads share; DN is 64 or 128,
-    DR 32 or 64, all bfloat16 or float16 (any strides). Returns [B, Sq, H, DN];
+    DR 32 or 64, all bfloat16 or float16 (any strides, tokens less than 2^24
+    elements apart). Returns [B, Sq, H, DN];
     ``scale`` is 1 / sqrt(DN + DR) unless given.
 
     ``lengths`` (int32 [B]) are the valid keys of each padded sequence, ``past``
@@ -293,8 +294,9 @@ def latent_cache_attention(q: Tensor, cache: Tensor, block_table: Tensor,
     position, lengths - Sq + i; one before the start comes back zero, as does
     an empty sequence. Table entries behind a sequence are not read. A length
     that the table cannot hold, or a page number that the cache does not have,
-    makes that sequence's outputs NaN. Up to 128 (query, head) pairs share one
-    pass over the cache; a few tokens at a time are what it is made for."""
+    makes that sequence's outputs NaN. All heads and queries of a sequence
+    share one pass over its tokens; a few queries at a time are what it is
+    made for."""
     run = _hip.latent_cache_attention if _use_hip(q) \
         else torch_ref.latent_cache_attention
     return run(q, cache, block_table, lengths, latent_dim, scale)
