@@ -13,6 +13,8 @@
 
 #include <c10/core/DeviceGuard.h>
 
+#include <algorithm>
+
 #include "common.h"
 #include "mfma_tiles.h"
 
@@ -44,6 +46,11 @@ struct InnerArgs {
     int M, K, rows_per_id, n_adapters, rank, rank_pad;
     int item_rows, item_blocks; // rows that blocks do not cross
     bool vec;                   // rows lie at multiples of 16 bytes
+    // up with its rows padded to whole chunks, or nullptr
+    const __bf16* up;           // [up_rows][rank]
+    __bf16* up_padded;          // [up_rows][chunks][8]
+    long up_rows;
+    int row_blocks;             // blocks behind these pad
 };
 
 __device__ __forceinline__ bf16x8 inner_load(const __bf16* p, int k, int K,
@@ -57,6 +64,20 @@ __device__ __forceinline__ bf16x8 inner_load(const __bf16* p, int k, int K,
             if (k + j < K) v[j] = p[k + j];
     }
     return v;
+}
+
+// The blocks behind a.row_blocks: rows of up as whole chunks of 8.
+__device__ __forceinline__ void pad_rows(const InnerArgs& a) {
+    if (blockIdx.y > 0) return;
+    const int chunks = (a.rank + 7) / 8;
+    const long count = a.up_rows * chunks;
+    const long step = (long)(gridDim.x - a.row_blocks) * blockDim.x;
+    for (long i = (long)(blockIdx.x - a.row_blocks) * blockDim.x
+                  + threadIdx.x; i < count; i += step) {
+        const long row = i / chunks;
+        reinterpret_cast<bf16x8*>(a.up_padded)[i] = inner_load(
+            a.up + row * a.rank, (int)(i - row * chunks) * 8, a.rank, false);
+    }
 }
 
 // x Phi(x) with Phi(-z) = exp(-z^2 / 2) r(z), z >= 0. r, the half of the
@@ -90,6 +111,7 @@ template <int NC, bool VEC>
 __global__ __launch_bounds__(256) void adapter_inner_kernel(InnerArgs a) {
     constexpr int DEPTH = 4;    // steps of 32 whose loads are on their way
     __shared__ float parts[4][NC][64][4];
+    if (blockIdx.x >= a.row_blocks) { pad_rows(a); return; }
     const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
     const int l15 = lane & 15, quad = lane >> 4;
     const int row0 = blockIdx.x * 16, col0 = blockIdx.y * 16 * NC;
@@ -187,6 +209,7 @@ void adapter_inner_tile_kernel(InnerArgs a) {
     constexpr int PIECES = (BN + BM) / 8 / (WN * WM);
     typedef TileVec<__bf16>::v8 v8;
     __shared__ __attribute__((aligned(256))) __bf16 lds[WK * BUFS * SLICE];
+    if (blockIdx.x >= a.row_blocks) { pad_rows(a); return; }
 
     const int tid = threadIdx.x, lane = tid & 63;
     const int l31 = lane & 31, hi = lane >> 5;
@@ -806,13 +829,15 @@ void inner_launch(const InnerArgs& a, dim3 grid) {
                            0, pe_current_stream(), a);
 }
 
-void adapter_inner(const InnerArgs& a) {
+void adapter_inner(InnerArgs a) {
     if (a.M <= STEP_ROWS) {
         hipLaunchKernelGGL(adapter_inner_step_kernel,
                            dim3(a.M, a.rank_pad / 16), dim3(256), 0,
                            pe_current_stream(), a);
         return;
     }
+    const int pads = a.up_padded == nullptr ? 0 : (int)std::min<long>(
+        256, (a.up_rows * ((a.rank + 7) / 8) + 1023) / 1024);
     // From about 2048 rows of rank 64 on, the way through LDS wins (12608
     // rows of 1280: rank 64 26 us against 10, rank 16 12 against 11; 3152
     // rows: rank 64 10 against 9; 1576 rows of 768, rank 8: 4.5 against 12).
@@ -821,19 +846,21 @@ void adapter_inner(const InnerArgs& a) {
         // blocks that end with their item have one adapter and read K once
         t.item_rows = a.rows_per_id >= 64 ? a.rows_per_id : a.M;
         t.item_blocks = (t.item_rows + 63) / 64;
-        const int rows = t.item_blocks * (a.M / t.item_rows);
+        t.row_blocks = t.item_blocks * (a.M / t.item_rows);
+        const int blocks = t.row_blocks + pads;
         if (a.rank <= 32)
             hipLaunchKernelGGL((adapter_inner_tile_kernel<1, 2, 2, 4>),
-                               dim3(rows, 1), dim3(256), 0,
+                               dim3(blocks, 1), dim3(256), 0,
                                pe_current_stream(), t);
         else
             hipLaunchKernelGGL((adapter_inner_tile_kernel<2, 2, 2, 4>),
-                               dim3(rows, a.rank_pad / 64), dim3(512), 0,
+                               dim3(blocks, a.rank_pad / 64), dim3(512), 0,
                                pe_current_stream(), t);
         return;
     }
     // columns a block: all of them up to 64, then 64 at a time
-    const dim3 grid((a.M + 15) / 16, (a.rank + 63) / 64);
+    a.row_blocks = (a.M + 15) / 16;
+    const dim3 grid(a.row_blocks + pads, (a.rank + 63) / 64);
     if (a.rank <= 16) inner_launch<1>(a, grid);
     else if (a.rank <= 32) inner_launch<2>(a, grid);
     else inner_launch<4>(a, grid);
@@ -934,12 +961,14 @@ torch::Tensor adapter_linear_op(
     const auto w = adapter_dense(weight);
     const auto down_c = adapter_dense(down);
     // The products of many rows read up 8 of the rank at a time. Ranks between
-    // are padded here: loads of single elements in each block cost more
-    // (12608 rows, 1280 to 5120 columns, rank 60: 253 us padded, 318 so; 1576
-    // rows, 768 to 2304, rank 4: 26 and 27).
-    const bool pad_up = M > STEP_ROWS && r % 8 != 0;
-    const auto up_c = pad_up ? at::constant_pad_nd(up, {0, 8 - r % 8})
-                             : adapter_dense(up);
+    // are padded, by the kernel of the inner values: loads of single elements
+    // by each block of the product cost more (12608 rows, 1280 to 5120
+    // columns, rank 60: 253 us padded, 318 so), two launches more as well
+    // (1000 rows, 320 to 700, rank 4: 18 us, 11 so).
+    const auto up_c = adapter_dense(up);
+    const bool pad_up = M > STEP_ROWS && n > 0 && r % 8 != 0;
+    const int64_t up_rank = pad_up ? (r + 7) / 8 * 8 : r;
+    auto up_padded = torch::empty({pad_up ? n : 0, N, up_rank}, x.options());
     const auto ids_c = ids.contiguous();
     const auto tensor_or_none = [](c10::optional<torch::Tensor>& t) {
         if (!t.has_value()) return (const __bf16*)nullptr;
@@ -959,11 +988,12 @@ torch::Tensor adapter_linear_op(
     a.M = M, a.N = N, a.K = K, a.act = act;
     a.vec = K % 8 == 0;
     a.ad.inner = reinterpret_cast<const __bf16*>(inner.data_ptr());
-    a.ad.up = reinterpret_cast<const __bf16*>(up_c.data_ptr());
+    a.ad.up = reinterpret_cast<const __bf16*>(
+        pad_up ? up_padded.data_ptr() : up_c.data_ptr());
     a.ad.row_ids = ids_c.data_ptr<int>();
     a.ad.rows_per_id = by_row ? 1 : M / x.size(0);
     a.ad.n_adapters = any ? n : 0;      // without any, no id is inside
-    a.ad.rank = up_c.size(2), a.ad.rank_pad = rank_pad;
+    a.ad.rank = up_rank, a.ad.rank_pad = rank_pad;
     if (any) {
         InnerArgs in = {};
         in.x = a.x;
@@ -979,6 +1009,10 @@ torch::Tensor adapter_linear_op(
         in.rows_per_id = a.ad.rows_per_id;
         in.rank_pad = rank_pad;
         in.vec = a.vec;
+        in.up = reinterpret_cast<const __bf16*>(up_c.data_ptr());
+        if (pad_up)
+            in.up_padded = reinterpret_cast<__bf16*>(up_padded.data_ptr());
+        in.up_rows = n * N;
         adapter_inner(in);
         HIP_CHECK_LAST();
     }
