@@ -337,11 +337,12 @@ void adapter_inner_tile_kernel(InnerArgs a) {
     }
 }
 
-// Few rows: a wave takes one row and 4 inner columns, a block 16 of them. The
-// matrix unit would be idle for want of rows; what counts is that all the
-// adapters' rows are on their way at once.
+// Few rows, or few of each adapter: a wave takes one row and 4 inner columns,
+// a block 16 of them. The matrix unit would be idle for want of rows; what
+// counts is that all the adapters' rows are on their way at once.
 __global__ __launch_bounds__(256) void adapter_inner_step_kernel(
         InnerArgs a) {
+    if (blockIdx.x >= a.row_blocks) { pad_rows(a); return; }
     const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
     const int row = blockIdx.x, col0 = blockIdx.y * 16 + wid * 4;
     int id = a.row_ids[row / a.rows_per_id];
@@ -830,14 +831,21 @@ void inner_launch(const InnerArgs& a, dim3 grid) {
 }
 
 void adapter_inner(InnerArgs a) {
-    if (a.M <= STEP_ROWS) {
+    const int pads = a.up_padded == nullptr ? 0 : (int)std::min<long>(
+        256, (a.up_rows * ((a.rank + 7) / 8) + 1023) / 1024);
+    // Up to 512 rows of rank 64, a wave for each row and 4 columns: it reads
+    // the row's adapter alone, where the matrix unit takes all adapters of 16
+    // rows in turn. Whole projection, 1280 to 1280 columns, rank 64, us with
+    // it and without, rows of one adapter and of 8 mixed: 256 rows 14 and 18,
+    // 18 and 62; 512 rows 17 and 18, 21 and 63; 1024 rows 23 and 20, 28 and
+    // 71; 768 to 768, rank 8, 512 rows: 12 and 11, 15 and 22.
+    if ((long)a.M * std::max(a.rank_pad, 64) <= 512 * 64) {
+        a.row_blocks = a.M;
         hipLaunchKernelGGL(adapter_inner_step_kernel,
-                           dim3(a.M, a.rank_pad / 16), dim3(256), 0,
+                           dim3(a.M + pads, a.rank_pad / 16), dim3(256), 0,
                            pe_current_stream(), a);
         return;
     }
-    const int pads = a.up_padded == nullptr ? 0 : (int)std::min<long>(
-        256, (a.up_rows * ((a.rank + 7) / 8) + 1023) / 1024);
     // From about 2048 rows of rank 64 on, the way through LDS wins (12608
     // rows of 1280: rank 64 26 us against 10, rank 16 12 against 11; 3152
     // rows: rank 64 10 against 9; 1576 rows of 768, rank 8: 4.5 against 12).

@@ -104,6 +104,8 @@ def test_adapter_matches_exact(device, shape, k, n, rank, count):
     ((8, 200), 128, 4100, 70, 3),
     ((3, 100), 64, 300, 1, 5),
     ((2, 90), 136, 70, 255, 2),
+    ((6, 400), 64, 90, 33, 4),       # inner values of each kernel
+    ((3, 512), 72, 40, 12, 7),
 ])
 def test_adapter_odd_ranks(device, shape, k, n, rank, count):
     x, w, down, up = make(shape, k, n, rank, count, device)
