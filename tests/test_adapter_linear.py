@@ -158,6 +158,26 @@ def test_adapter_isolation(device, shape):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("shape,rank", [
+    ((4, 150), 16), ((7, 300), 64), ((5, 1000), 16), ((30, 20), 12),
+])
+def test_adapter_isolation_of_many_rows(device, shape, rank):
+    """The same where tiles of the matrix unit hold rows of several
+    requests."""
+    x, w, down, up = make(shape, 72, 136, rank, 3, device)
+    ids = (torch.arange(shape[0]) % 4 - 1).int().to(device)
+    want = ops.adapter_linear(x, w, down, up, ids)
+    down[1, 3, 5] = float("inf")
+    up[1] = float("nan")
+    x[2, 1, 0] = float("nan")
+    out = ops.adapter_linear(x, w, down, up, ids)
+    clean = torch.ones(shape[0], dtype=torch.bool)
+    clean[2::4] = False             # requests of adapter 1
+    assert torch.equal(out[clean], want[clean])
+    assert out[2].isnan().all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("rows", [4, 96])
 def test_adapter_gelu_range(device, rows):
     """The activation alone over its range: an identity projection, whose
@@ -260,3 +280,23 @@ def test_adapter_graph(shape):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, ops.adapter_linear(x, w, down, up, ids))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape,rank", [((8, 1), 16), ((3, 100), 12),
+                                        ((8, 197), 64)])
+def test_adapter_streams(shape, rank):
+    """Calls on two streams at once, whose inner values are their own."""
+    sets = [make(shape, 512, 640, rank, 4, "cuda", seed=i) for i in range(2)]
+    ids = (torch.arange(shape[0]) % 5 - 1).int().cuda()
+    want = [ops.adapter_linear(*s, ids, act="gelu") for s in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        outs = []
+        for stream, s in zip(streams, sets):
+            with torch.cuda.stream(stream):
+                outs.append(ops.adapter_linear(*s, ids, act="gelu"))
+        torch.cuda.synchronize()
+        for out, ref in zip(outs, want):
+            assert torch.equal(out, ref)

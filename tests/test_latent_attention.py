@@ -274,6 +274,21 @@ def test_expanded_far_sequences(sq, sk):
 
 
 @pytest.mark.gpu
+def test_expanded_refuses_far_tokens():
+    q, kv, k_rope = make_expanded(1, 2, 2, 1, 64, 32, torch.float16, "cuda")
+    room = torch.zeros(2 ** 24 + 4096, dtype=torch.float16, device="cuda")
+    for step, fits in ((2 ** 24 - 8, True), (2 ** 24, False)):
+        far = room.as_strided(kv.shape, (step, step, 128, 1))
+        far.copy_(kv)
+        if fits:
+            assert torch.equal(ops.latent_attention(q, far, k_rope),
+                               ops.latent_attention(q, kv, k_rope))
+        else:
+            with pytest.raises(ValueError):
+                ops.latent_attention(q, far, k_rope)
+
+
+@pytest.mark.gpu
 def test_expanded_shared_range_graphs():
     """The partial sums are a graph's own: two graphs and eager calls on
     another stream, in turn and at once."""
@@ -398,6 +413,21 @@ def test_cache_many_and_one_long(device, h, page):
                                      scale=0.06)
     check(out, *cache_exact(q, cache, table, lengths, 256, 0.06),
           torch.float16)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_cache_shared_pages(device):
+    """Sequences with a common beginning share its pages, and a page may
+    stand in a sequence twice."""
+    lengths = [40, 33, 50]
+    q, cache, table, n = make_cache(lengths, 2, 16, 256, 32, 16,
+                                    torch.bfloat16, device)
+    table[1, :2] = table[0, :2]
+    table[2, 1] = table[2, 0]
+    out = ops.latent_cache_attention(q, cache, table, n, latent_dim=256,
+                                     scale=0.06)
+    check(out, *cache_exact(q, cache, table, lengths, 256, 0.06),
+          torch.bfloat16)
 
 
 @pytest.mark.gpu
