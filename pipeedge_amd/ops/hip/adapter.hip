@@ -379,9 +379,11 @@ __global__ __launch_bounds__(256) void adapter_inner_step_kernel(
 
 // The whole projection of few rows. Bound by reading W: a block takes 16
 // columns and all rows, its waves a part of K each, so that 4096 columns are
-// on 256 CUs and every wave has its loads on the way before it needs one.
+// on 256 CUs and every wave has its loads on the way before it needs one (cold,
+// whole projection, us with 4 waves and with 8: 5120 to 1280 columns, 8 rows 28
+// and 24; 1024 to 4096, 8 rows 13.4 and 13.4, 64 rows 18.6 and 16.6).
 // The adapters' products are a short dot product for each output.
-constexpr int STEP_WAVES = 4;
+constexpr int STEP_WAVES = 8;
 
 template <int NM>               // groups of 16 rows
 __global__ __launch_bounds__(64 * STEP_WAVES) void adapter_step_kernel(
