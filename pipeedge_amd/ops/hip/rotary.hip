@@ -274,6 +274,11 @@ std::tuple<torch::Tensor, c10::optional<torch::Tensor>> rotary_op(
                               "rotary_: q and k overlap");
             k_out = *k;
         }
+        // a graph that has saved either has to find out, as after torch's own
+        // operators (tensors made in inference mode carry no version)
+        for (const auto& x : {q, k_out})
+            if (x.defined() && !x.is_inference())
+                x.unsafeGetTensorImpl()->bump_version();
     } else {
         q_out = torch::empty(q.sizes(), q.options());
         if (k.has_value()) k_out = torch::empty(k->sizes(), k->options());

@@ -266,3 +266,23 @@ def test_rotary_streams_and_graph():
         torch.cuda.synchronize()
         want = ops.rotary(q, pos, freqs, k)
         assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_rotary_in_place_is_seen_by_autograd(device):
+    """A graph that saved a tensor refuses to go back once it was turned."""
+    freqs = ops.rotary_frequencies(8, device=device)
+    pos = torch.arange(6, device=device).reshape(2, 3)
+    q = torch.randn(2, 3, 4, 8, device=device)
+    k = torch.randn(2, 3, 1, 8, device=device)
+    for kw in (dict(k=k), {}):
+        for x in (q, k)[:1 + len(kw)]:
+            w = torch.ones_like(x, requires_grad=True)
+            loss = (w * x).sum()
+            ops.rotary_(q, pos, freqs, **kw)
+            with pytest.raises(RuntimeError):
+                loss.backward()
+    with torch.inference_mode():
+        x = q.clone()
+        ops.rotary_(x, pos, freqs)
+    assert torch.equal(x, ops.rotary(q, pos, freqs))
