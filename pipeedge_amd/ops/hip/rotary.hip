@@ -14,7 +14,9 @@
 // 24 heads of 64 bf16, 77 MB: 14.7 us).
 #include <torch/extension.h>
 
-#include <ATen/MemoryOverlap.h>
+#include <algorithm>
+#include <vector>
+
 #include <c10/core/DeviceGuard.h>
 
 #include "common.h"
@@ -190,6 +192,84 @@ torch::Tensor rotary_view4(const torch::Tensor& x, const char* name) {
                    sizes[x.dim() - 1]});
 }
 
+// Two heads' columns that share memory would be turned twice, in no order. A
+// head's turned columns are one range of bytes, so the question is whether
+// some sum of strides, each times a number in its limits, comes within that
+// range's length of the distance between two heads.
+struct RotaryStep {
+    int64_t stride, low, high;
+};
+
+// Whether target - sum of number x stride can lie within reach of zero,
+// `nonzero`: with a number other than zero. Steps by falling stride, so that
+// nested layouts leave one or two numbers to try for each; what takes more
+// than `tries` counts as yes.
+bool rotary_reaches(const std::vector<RotaryStep>& steps, size_t at,
+                    int64_t target, int64_t reach, bool nonzero, int& tries) {
+    if (--tries < 0) return true;
+    if (at == steps.size()) return !nonzero && std::abs(target) <= reach;
+    int64_t low = -reach, high = reach;     // of what the rest can add
+    for (size_t i = at + 1; i < steps.size(); ++i) {
+        low += steps[i].low * steps[i].stride;
+        high += steps[i].high * steps[i].stride;
+    }
+    const int64_t s = steps[at].stride;
+    const auto down = [s](int64_t v) {
+        return v >= 0 ? v / s : -((-v + s - 1) / s);
+    };
+    const int64_t first = std::max(steps[at].low, -down(high - target));
+    const int64_t last = std::min(steps[at].high, down(target - low));
+    for (int64_t n = first; n <= last; ++n)
+        if (rotary_reaches(steps, at + 1, target - n * s, reach,
+                           nonzero && n == 0, tries))
+            return true;
+    return false;
+}
+
+constexpr int ROTARY_TRIES = 1 << 14;
+
+// both over the tensors' `width` turned columns, of equal place in the heads
+bool rotary_overlaps_itself(const torch::Tensor& x, int64_t width) {
+    std::vector<RotaryStep> steps;
+    for (int64_t d = 0; d + 1 < x.dim(); ++d) {
+        if (x.size(d) == 0) return false;
+        if (x.size(d) == 1) continue;
+        if (x.stride(d) == 0) return true;
+        steps.push_back({x.stride(d), 1 - x.size(d), x.size(d) - 1});
+    }
+    std::sort(steps.begin(), steps.end(), [](const auto& a, const auto& b) {
+        return a.stride > b.stride;
+    });
+    int tries = ROTARY_TRIES;
+    return rotary_reaches(steps, 0, 0, width - 1, true, tries);
+}
+
+bool rotary_overlap(const torch::Tensor& q, const torch::Tensor& k,
+                    int64_t width) {
+    const int64_t size = q.element_size();
+    std::vector<RotaryStep> steps;
+    for (const auto* x : {&q, &k})
+        for (int64_t d = 0; d + 1 < x->dim(); ++d) {
+            if (x->size(d) == 0) return false;
+            if (x->size(d) == 1) continue;
+            const int64_t stride = x->stride(d) * size, n = x->size(d) - 1;
+            auto same = std::find_if(
+                steps.begin(), steps.end(),
+                [stride](const auto& s) { return s.stride == stride; });
+            if (same == steps.end())
+                same = steps.insert(same, {stride, 0, 0});
+            (x == &q ? same->high : same->low) += x == &q ? n : -n;
+        }
+    std::sort(steps.begin(), steps.end(), [](const auto& a, const auto& b) {
+        return a.stride > b.stride;
+    });
+    int tries = ROTARY_TRIES;
+    return rotary_reaches(
+        steps, 0, static_cast<const char*>(k.data_ptr())
+                      - static_cast<const char*>(q.data_ptr()),
+        width * size - 1, false, tries);
+}
+
 template <typename T, int VEC, bool INTERLEAVED>
 void rotary_launch(const RotaryArgs& a, bool wide, int blocks, size_t lds) {
     if (wide)
@@ -261,16 +341,13 @@ std::tuple<torch::Tensor, c10::optional<torch::Tensor>> rotary_op(
     }
     torch::Tensor q_out = q, k_out;
     if (in_place) {
-        TORCH_CHECK_VALUE(at::has_internal_overlap(q) !=
-                          at::MemOverlap::Yes &&
-                          (!k.has_value() || at::has_internal_overlap(*k) !=
-                           at::MemOverlap::Yes),
+        const int64_t width = 2 * pairs;
+        TORCH_CHECK_VALUE(!rotary_overlaps_itself(q, width) &&
+                          !(k.has_value() &&
+                            rotary_overlaps_itself(*k, width)),
                           "rotary_: a tensor overlaps itself");
         if (k.has_value()) {
-            const auto lap = at::get_overlap_status(q, *k);
-            TORCH_CHECK_VALUE(q.data_ptr() != k->data_ptr() &&
-                              lap != at::MemOverlapStatus::Full &&
-                              lap != at::MemOverlapStatus::Partial,
+            TORCH_CHECK_VALUE(!rotary_overlap(q, *k, width),
                               "rotary_: q and k overlap");
             k_out = *k;
         }

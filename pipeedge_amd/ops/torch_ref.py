@@ -13,7 +13,7 @@ k-contiguous per row, so A- and B-fragments alike stage through LDS with
 (cdna_hip_programming.md section 5).
 """
 import math
-from typing import Optional, Tuple
+from typing import Dict, List, Optional, Tuple
 
 import torch
 from torch import Tensor
@@ -112,6 +112,53 @@ def _check_inference(op: str, *tensors: Optional[Tensor]):
         raise ValueError(f"{op}: inference only, an input requires a gradient")
 
 
+def _reaches(steps: List[Tuple[int, int, int]], target: int, reach: int,
+             nonzero: bool, tries: List[int]) -> bool:
+    """Whether ``target`` less a sum of number x stride, with each number in
+    its limits, can lie within ``reach`` of zero; ``nonzero``: with a number
+    other than zero. ``steps`` by falling stride; more than ``tries`` is yes."""
+    tries[0] -= 1
+    if tries[0] < 0:
+        return True
+    if not steps:
+        return not nonzero and abs(target) <= reach
+    (stride, low, high), rest = steps[0], steps[1:]
+    rest_low = sum(lo * s for s, lo, _ in rest) - reach
+    rest_high = sum(hi * s for s, _, hi in rest) + reach
+    first = max(low, -((rest_high - target) // stride))
+    last = min(high, (target - rest_low) // stride)
+    return any(_reaches(rest, target - n * stride, reach,
+                        nonzero and n == 0, tries)
+               for n in range(first, last + 1))
+
+
+def _overlaps_itself(x: Tensor, width: int) -> bool:
+    """Whether two heads of ``x`` share any of ``width`` adjacent columns."""
+    dims = [(st, n) for st, n in zip(x.stride()[:-1], x.shape[:-1]) if n != 1]
+    if any(n == 0 for _, n in dims):
+        return False
+    if any(st == 0 for st, _ in dims):
+        return True
+    steps = sorted(((st, 1 - n, n - 1) for st, n in dims), reverse=True)
+    return _reaches(steps, 0, width - 1, True, [1 << 14])
+
+
+def _overlap(q: Tensor, k: Tensor, width: int) -> bool:
+    """The same for a head of ``q`` and one of ``k``."""
+    size = q.element_size()
+    limits: Dict[int, List[int]] = {}
+    for x, at, sign in ((q, 1, 1), (k, 0, -1)):
+        if 0 in x.shape[:-1]:
+            return False
+        for st, n in zip(x.stride()[:-1], x.shape[:-1]):
+            if n > 1:
+                limits.setdefault(st * size, [0, 0])[at] += sign * (n - 1)
+    steps = sorted(((st, lo, hi) for st, (lo, hi) in limits.items()),
+                   reverse=True)
+    return _reaches(steps, k.data_ptr() - q.data_ptr(), width * size - 1,
+                    False, [1 << 14])
+
+
 def check_rotary(q: Tensor, positions: Tensor, freqs: Tensor,
                  k: Optional[Tensor], offset: int, in_place: bool):
     """The argument checks of the rotary kernel, for the CPU path."""
@@ -135,9 +182,6 @@ def check_rotary(q: Tensor, positions: Tensor, freqs: Tensor,
         if x.shape[-1] > 1 and x.stride(-1) != 1:
             raise ValueError(f"rotary: {name} must be contiguous in its "
                              "last dimension")
-        if in_place and any(n > 1 and st == 0
-                            for n, st in zip(x.shape, x.stride())):
-            raise ValueError("rotary_: a tensor overlaps itself")
     pairs, dim = freqs.numel(), q.shape[-1]
     if pairs < 1 or offset < 0 or offset + 2 * pairs > dim:
         raise ValueError(f"rotary: columns {offset} to {offset + 2 * pairs} "
@@ -151,7 +195,11 @@ def check_rotary(q: Tensor, positions: Tensor, freqs: Tensor,
         if k.dim() != q.dim() or k.shape[-1] != dim \
                 or k.shape[:-2] != q.shape[:-2]:
             raise ValueError("rotary: k must match q except in its heads")
-        if in_place and k.numel() and k.data_ptr() == q.data_ptr():
+    if in_place:
+        if any(t is not None and _overlaps_itself(t, 2 * pairs)
+               for t in (q, k)):
+            raise ValueError("rotary_: a tensor overlaps itself")
+        if k is not None and _overlap(q, k, 2 * pairs):
             raise ValueError("rotary_: q and k overlap")
 
 

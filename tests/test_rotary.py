@@ -2,6 +2,7 @@
 head, strides, far positions, in-place views, refusals. Every case runs on
 the CPU path; with a GPU the same cases run on the HIP kernel."""
 import math
+import random
 
 import pytest
 import torch
@@ -286,3 +287,76 @@ def test_rotary_in_place_is_seen_by_autograd(device):
         x = q.clone()
         ops.rotary_(x, pos, freqs)
     assert torch.equal(x, ops.rotary(q, pos, freqs))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("seed", range(12))
+def test_rotary_in_place_overlap(device, seed):
+    """In place, every layout whose turned columns are apart is turned, every
+    other one is refused: random views of one storage, addresses counted."""
+    rng = random.Random(seed)
+    freqs = ops.rotary_frequencies(4, device=device)
+    turned = 0
+    for _ in range(40):
+        b, s = rng.randint(1, 3), rng.randint(1, 4)
+        base = torch.randn(2000, device=device)
+        nested = rng.random() < 0.7
+        views, places = [], []
+        strides = None
+        for heads in (rng.randint(1, 3), rng.randint(1, 3)):
+            if strides is None or rng.random() < 0.4:
+                strides = [rng.randint(0, 40) for _ in range(3)]
+                if nested:
+                    strides[2] = rng.randint(4, 9)
+                    strides[1] = strides[2] * 3 + rng.randint(0, 30)
+                    strides[0] = strides[1] * s + rng.randint(0, 20)
+            start = rng.randint(0, 60)
+            views.append(base.as_strided((b, s, heads, 6), strides + [1],
+                                         start))
+            # columns 1 to 4 of each head
+            places.append([start + i * strides[0] + j * strides[1]
+                           + h * strides[2] + c for i in range(b)
+                           for j in range(s) for h in range(heads)
+                           for c in range(1, 5)])
+        pos = torch.randint(0, 99, (b, s), device=device)
+        q, k = views
+        own = [len(set(p)) < len(p) for p in places]
+        both = bool(set(places[0]) & set(places[1]))
+        for args, bad in (((q, pos, freqs), own[0]),
+                          ((q, pos, freqs, k), any(own) or both)):
+            before = base.clone()
+            if bad:
+                with pytest.raises(ValueError):
+                    ops.rotary_(*args, offset=1)
+                assert torch.equal(base, before)
+                continue
+            want = base.clone()
+            for x in args[:1] + args[3:]:
+                w = want.as_strided(x.shape, x.stride(), x.storage_offset())
+                w[..., 1:5] = ops.rotary(x, pos, freqs, offset=1)[..., 1:5]
+            ops.rotary_(*args, offset=1)
+            assert torch.equal(base, want)
+            turned += 1
+    assert turned >= 5
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_rotary_in_place_keys_behind_queries(device):
+    """Parts of one packed tensor, apart by heads, by columns and by tokens;
+    and the same parts one head, one column, one token too long."""
+    freqs = ops.rotary_frequencies(32, device=device)
+    pos = torch.arange(14, device=device).reshape(2, 7)
+    base = torch.randn(2, 9, 6, 96, device=device, dtype=torch.bfloat16)
+    x = base[:, :7]
+    for q, k in ((x[:, :, :4], x[:, :, 4:]), (x[:, :, ::2], x[:, :, 1::2]),
+                 (x[..., :48], x[..., 48:]), (x[..., :40], x[..., 32:72]),
+                 (base[:, :7, :3], base[:, 2:, 3:])):
+        want = ops.rotary(q, pos, freqs, k)
+        width = slice(0, 32)
+        ops.rotary_(q, pos, freqs, k)
+        assert torch.equal(q[..., width], want[0][..., width])
+        assert torch.equal(k[..., width], want[1][..., width])
+    for q, k in ((x[:, :, :4], x[:, :, 3:]), (x[..., :40], x[..., 31:71]),
+                 (base[:, :7], base[:, 2:]), (x, x), (x, x[..., :96])):
+        with pytest.raises(ValueError):
+            ops.rotary_(q, pos, freqs, k)
