@@ -360,3 +360,17 @@ def test_rotary_in_place_keys_behind_queries(device):
                  (base[:, :7], base[:, 2:]), (x, x), (x, x[..., :96])):
         with pytest.raises(ValueError):
             ops.rotary_(q, pos, freqs, k)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_rotary_in_place_empty(device):
+    """No tokens, no query heads, no key heads: the others are turned."""
+    freqs = ops.rotary_frequencies(8, device=device)
+    for lead, heads in (((2, 0), (4, 1)), ((0, 3), (4, 1)), ((2, 3), (0, 1)),
+                        ((2, 3), (1, 0)), ((2, 3), (0, 0))):
+        q, k = (torch.randn(*lead, h, 8, device=device) for h in heads)
+        pos = torch.ones(lead, dtype=torch.int64, device=device)
+        want = ops.rotary(q, pos, freqs, k)
+        got = ops.rotary_(q, pos, freqs, k)
+        assert got[0] is q and got[1] is k
+        assert torch.equal(q, want[0]) and torch.equal(k, want[1])
