@@ -14,6 +14,7 @@
 // 24 heads of 64 bf16, 77 MB: 14.7 us).
 #include <torch/extension.h>
 
+#include <ATen/TensorUtils.h>
 #include <algorithm>
 #include <vector>
 
@@ -176,20 +177,30 @@ bool rotary_aligned(const torch::Tensor& x, int vec) {
     return true;
 }
 
-// [.., H, D] as [B, S, H, D] over the same memory
-torch::Tensor rotary_view4(const torch::Tensor& x, const char* name) {
+// the sizes of [.., H, D] as [B, S, H, D]
+std::vector<int64_t> rotary_sizes4(const torch::Tensor& x) {
+    std::vector<int64_t> sizes(4, 1);
+    for (int64_t d = 0; d < x.dim(); ++d)
+        sizes[std::max<int64_t>(d + 4 - x.dim(), 0)] *= x.size(d);
+    return sizes;
+}
+
+// whether that is a view, the leading dimensions being one in memory
+bool rotary_is_view4(const torch::Tensor& x) {
+    return at::detail::computeStride(x.sizes(), x.strides(),
+                                     rotary_sizes4(x)).has_value();
+}
+
+// over the same memory where it is, else a copy
+torch::Tensor rotary_as4(const torch::Tensor& x) {
+    return x.dim() == 4 ? x : x.reshape(rotary_sizes4(x));
+}
+
+void rotary_check(const torch::Tensor& x, const char* name) {
     TORCH_CHECK_VALUE(x.dim() >= 2, "rotary: ", name,
                       " must be [.., heads, dim]");
     TORCH_CHECK_VALUE(x.size(-1) <= 1 || x.stride(-1) == 1, "rotary: ", name,
                       " must be contiguous in its last dimension");
-    if (x.dim() == 2) return x.unsqueeze(0).unsqueeze(0);
-    if (x.dim() == 3) return x.unsqueeze(0);
-    if (x.dim() == 4) return x;
-    auto sizes = x.sizes();
-    int64_t lead = 1;
-    for (int64_t d = 0; d + 3 < x.dim(); ++d) lead *= sizes[d];
-    return x.view({lead, sizes[x.dim() - 3], sizes[x.dim() - 2],
-                   sizes[x.dim() - 1]});
 }
 
 // Two heads' columns that share memory would be turned twice, in no order. A
@@ -316,18 +327,17 @@ std::tuple<torch::Tensor, c10::optional<torch::Tensor>> rotary_op(
                         (q.requires_grad() ||
                          (k.has_value() && k->requires_grad()))),
                       "rotary: inference only, an input requires a gradient");
+    rotary_check(q, "q");
     const int64_t pairs = freqs.numel(), dim = q.size(-1);
     TORCH_CHECK_VALUE(pairs >= 1 && offset >= 0 && offset + 2 * pairs <= dim,
                       "rotary: columns ", offset, " to ", offset + 2 * pairs,
                       " do not fit a head of ", dim);
     TORCH_CHECK_VALUE(pairs <= 1024, "rotary: more than 2048 rotated columns");
     TORCH_CHECK_VALUE(positions.sizes() ==
-                      q.sizes().slice(0, std::max<int64_t>(q.dim() - 2, 0)),
+                      q.sizes().slice(0, q.dim() - 2),
                       "rotary: positions must be one a token, shape ",
-                      q.sizes().slice(0, std::max<int64_t>(q.dim() - 2, 0)),
+                      q.sizes().slice(0, q.dim() - 2),
                       ", got ", positions.sizes());
-    const auto q4 = rotary_view4(q, "q");
-    torch::Tensor k4;
     if (k.has_value()) {
         TORCH_CHECK_TYPE(k->scalar_type() == dtype,
                          "rotary: q and k must have one type");
@@ -337,7 +347,7 @@ std::tuple<torch::Tensor, c10::optional<torch::Tensor>> rotary_op(
                           k->sizes().slice(0, q.dim() - 2) ==
                           q.sizes().slice(0, q.dim() - 2),
                           "rotary: k must match q except in its heads");
-        k4 = rotary_view4(*k, "k");
+        rotary_check(*k, "k");
     }
     torch::Tensor q_out = q, k_out;
     if (in_place) {
@@ -363,15 +373,28 @@ std::tuple<torch::Tensor, c10::optional<torch::Tensor>> rotary_op(
     c10::optional<torch::Tensor> k_result;
     if (k.has_value()) k_result = k_out;
 
+    if (in_place && q.dim() > 4 &&
+        !(rotary_is_view4(q) && (!k.has_value() || rotary_is_view4(*k)))) {
+        // leading dimensions that are not one in memory: each by itself
+        for (int64_t i = 0; i < q.size(0); ++i)
+            rotary_op(q.select(0, i), positions.select(0, i), freqs,
+                      k.has_value()
+                          ? c10::optional<torch::Tensor>(k->select(0, i))
+                          : c10::nullopt,
+                      interleaved, offset, inverse, scale, true);
+        return {q_out, k_result};
+    }
+    const auto q4 = rotary_as4(q);
+    const auto k4 = k.has_value() ? rotary_as4(*k) : torch::Tensor();
     const int64_t tokens = q4.size(0) * q4.size(1);
     const int64_t heads = q4.size(2) + (k.has_value() ? k4.size(2) : 0);
     if (tokens == 0 || heads == 0) return {q_out, k_result};
     // the kernel's division by a reciprocal is exact below 2^32 / dim
     TORCH_CHECK_VALUE(tokens < (1L << 31) && heads * dim * dim < (1L << 32),
                       "rotary: too many tokens or columns");
-    const auto q4_out = in_place ? q4 : rotary_view4(q_out, "q");
+    const auto q4_out = in_place ? q4 : rotary_as4(q_out);
     const auto k4_out = !k.has_value() || in_place
-        ? k4 : rotary_view4(k_out, "k");
+        ? k4 : rotary_as4(k_out);
 
     const int wide = dtype == torch::kFloat ? 4 : 8;
     bool vec = pairs % wide == 0 && offset % wide == 0 && dim % wide == 0 &&

@@ -374,3 +374,27 @@ def test_rotary_in_place_empty(device):
         got = ops.rotary_(q, pos, freqs, k)
         assert got[0] is q and got[1] is k
         assert torch.equal(q, want[0]) and torch.equal(k, want[1])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_rotary_leading_dimensions(device):
+    """Five and six dimensions whose leading ones are not one in memory."""
+    freqs = ops.rotary_frequencies(16, device=device)
+    x = torch.randn(3, 2, 5, 6, 16, device=device)
+    y = torch.randn(2, 4, 3, 5, 6, 16, device=device)
+    for x, pos in ((x.transpose(0, 1), torch.randint(0, 99, (2, 3, 5))),
+                   (x[:, :1], torch.randint(0, 99, (3, 1, 5))),
+                   (y.permute(2, 0, 1, 3, 4, 5),
+                    torch.randint(0, 99, (3, 2, 4, 5))),
+                   (y[:, :, :2, ::2], torch.randint(0, 99, (2, 4, 2, 3)))):
+        pos = pos.to(device)
+        for q, k in ((x[..., :4, :], x[..., 4:, :]),
+                     (x[..., :4, :], x[..., 4:, :].contiguous()),
+                     (x[..., :4, :].contiguous(), x[..., 4:, :])):
+            want = ops.rotary(q.contiguous(), pos, freqs, k.contiguous())
+            out = ops.rotary(q, pos, freqs, k)
+            assert all(torch.equal(a, b) for a, b in zip(out, want))
+            assert torch.equal(ops.rotary(q, pos, freqs), want[0])
+            got = ops.rotary_(q, pos, freqs, k)
+            assert got[0] is q and got[1] is k
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
