@@ -324,7 +324,7 @@ std::tuple<torch::Tensor, c10::optional<torch::Tensor>> rotary_op(
                       freqs.device() == q.device(),
                       "rotary: tensors on different devices");
     TORCH_CHECK_VALUE(!(at::GradMode::is_enabled() &&
-                        (q.requires_grad() ||
+                        (q.requires_grad() || freqs.requires_grad() ||
                          (k.has_value() && k->requires_grad()))),
                       "rotary: inference only, an input requires a gradient");
     rotary_check(q, "q");

@@ -173,7 +173,7 @@ def check_rotary(q: Tensor, positions: Tensor, freqs: Tensor,
     if any(t is not None and t.device != q.device
            for t in (positions, freqs, k)):
         raise ValueError("rotary: tensors on different devices")
-    _check_inference("rotary", q, k)
+    _check_inference("rotary", q, k, freqs)
     for name, x in (("q", q), ("k", k)):
         if x is None:
             continue

@@ -398,3 +398,16 @@ def test_rotary_leading_dimensions(device):
             got = ops.rotary_(q, pos, freqs, k)
             assert got[0] is q and got[1] is k
             assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_rotary_refuses_gradients_of_frequencies(device):
+    q = torch.randn(2, 3, 4, 16, device=device)
+    pos = torch.arange(6, device=device).reshape(2, 3)
+    freqs = ops.rotary_frequencies(16, device=device).requires_grad_()
+    for op in (ops.rotary, ops.rotary_):
+        with pytest.raises(ValueError):
+            op(q, pos, freqs)
+    with torch.no_grad():
+        out = ops.rotary(q, pos, freqs)
+    assert torch.equal(out, ops.rotary(q, pos, freqs.detach()))
