@@ -277,9 +277,12 @@ __global__ __launch_bounds__(256, 2) void latent_attention_kernel(
             #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 typename TileVec<T>::v4 o;
+                // a row that sees nothing is zero, also where its zero weights
+                // met values that are not finite
                 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    o[j] = (T)(acc[n][g * 4 + j] * inv);
+                    o[j] = (T)(total == 0.0f ? 0.0f
+                                             : acc[n][g * 4 + j] * inv);
                 *reinterpret_cast<typename TileVec<T>::v4*>(
                     out + n * 32 + g * 8) = o;
             }

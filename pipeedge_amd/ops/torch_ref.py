@@ -308,6 +308,8 @@ def latent_attention(q: Tensor, kv: Tensor, k_rope: Tensor, scale: float,
                           full.transpose(-1, -2)) * scale
     weight = _softmax_seen(scores, seen.unsqueeze(1))
     out = torch.matmul(weight, heads[..., nope:].contiguous())
+    # also where zero weights met values that are not finite
+    out = out.masked_fill(~seen.any(-1).reshape(b, 1, sq, 1), 0.0)
     return out.transpose(1, 2).contiguous().to(q.dtype)
 
 

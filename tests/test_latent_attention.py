@@ -151,6 +151,32 @@ def test_expanded_long_keys(device, dtype, causal, sq, sk, h, nope, rope,
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("sq,sk,length,past", [
+    (150, 150, 100, 0),              # padding in a tile with live queries
+    (40, 40, 30, -9),                # queries before the start
+    (3, 1500, 1400, 1398),           # the keys in parts
+])
+def test_expanded_padding_stays_zero(device, causal, sq, sk, length, past):
+    """Queries outside their sequence are zero also where values inside it
+    are not finite."""
+    q, kv, k_rope = make_expanded(2, sq, sk, 2, 64, 32, torch.bfloat16,
+                                  device)
+    kv[1, 5, 1, 70] = math.inf
+    kv[1, length - 1, 0, 80] = math.nan
+    n = torch.full((2,), length, dtype=torch.int32, device=device)
+    p = torch.full((2,), past, dtype=torch.int32, device=device)
+    out = ops.latent_attention(q, kv, k_rope, causal=causal, lengths=n,
+                               past=p)
+    at = past + torch.arange(sq, device=device)
+    outside = (at < 0) | (at >= length)
+    assert outside.any() and not out[:, outside].any()
+    assert out[0].isfinite().all() and out[0, ~outside].any(-1).all()
+    last = int((~outside).nonzero().max())
+    assert not out[1, last, 1, 6].isfinite() and out[1, last, 0, 16].isnan()
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_expanded_strides(device):
     """Views: heads first, part of wider rows, misaligned storage."""
     dtype = torch.float16
