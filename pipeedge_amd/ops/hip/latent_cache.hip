@@ -517,9 +517,12 @@ void latent_cache_kernel(CacheArgs a) {
                          + ((long)seq * a.rows + row) * R + quad * 4;
                 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
+                    // a row that sees nothing is zero, also where its zero
+                    // weights met values that are not finite
                     typename TileVec<T>::v4 o;
                     #pragma unroll
-                    for (int j = 0; j < 4; ++j) o[j] = (T)(acc[n][j] * inv);
+                    for (int j = 0; j < 4; ++j)
+                        o[j] = (T)(sum == 0.0f ? 0.0f : acc[n][j] * inv);
                     *reinterpret_cast<typename TileVec<T>::v4*>(
                         out + n * 16) = o;
                 }
@@ -642,7 +645,8 @@ __global__ __launch_bounds__(256) void latent_cache_join_kernel(
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     v4 o;
     #pragma unroll
-    for (int j = 0; j < 4; ++j) o[j] = (T)(all[j] * inv);
+    for (int j = 0; j < 4; ++j)
+        o[j] = (T)(sum == 0.0f ? 0.0f : all[j] * inv);
     *reinterpret_cast<v4*>(out) = o;
 }
 

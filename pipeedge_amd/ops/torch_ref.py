@@ -368,6 +368,8 @@ def latent_cache_attention(q: Tensor, cache: Tensor, block_table: Tensor,
         seen = place <= at.reshape(sq, 1, 1)
         weight = _softmax_seen(scores, seen.expand(sq, h, n))
         out[i] = torch.matmul(weight, tokens[:, :latent_dim]).to(q.dtype)
+        # also where zero weights met values that are not finite
+        out[i, at < 0] = 0.0
     return out
 
 

@@ -493,6 +493,25 @@ def test_cache_peaked_scores(device, dtype):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("h,page", [(4, 16), (10, 7), (40, 64)])
+def test_cache_before_the_start_stays_zero(device, h, page):
+    """Queries before their sequence's start are zero also where what is
+    cached is not finite, in whole sequences and in joined ones."""
+    lengths = [2, 300, 5]
+    q, cache, table, n = make_cache(lengths, 303, h, 256, 32, page,
+                                    torch.bfloat16, device)
+    for i in (0, 1):
+        cache[table[i, 0].long(), 1, 7] = math.nan
+    out = ops.latent_cache_attention(q, cache, table, n, latent_dim=256,
+                                     scale=0.1)
+    for i, length in enumerate(lengths):
+        assert not out[i, :303 - length].any()
+        assert out[i, 303 - length:].any(-1).all()
+        assert out[i, -1, :, 7].isnan().all() == (i < 2)
+    assert out[2].isfinite().all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_cache_strided(device):
     """A layer's slice of a larger cache, queries with heads first, a table
     that is part of a wider one."""
