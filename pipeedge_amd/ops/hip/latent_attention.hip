@@ -21,6 +21,7 @@
 #include <torch/extension.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include <c10/core/DeviceGuard.h>
 
@@ -386,8 +387,12 @@ torch::Tensor latent_attention_op(
                       kv.size(2) == H && k_rope.size(1) == Sk,
                       "latent_attention: q ", q.sizes(), ", kv ", kv.sizes(),
                       " and k_rope ", k_rope.sizes(), " do not match");
-    TORCH_CHECK_VALUE(scale > 0.0 && std::isfinite(scale),
-                      "latent_attention: scale must be positive");
+    // the kernel's scale, in powers of two; zero or infinite in 32 bits it
+    // would turn hidden scores into NaN
+    const float scale2 = scale * 1.4426950408889634;
+    TORCH_CHECK_VALUE(scale2 > 0.0f && std::isnormal(scale2),
+                      "latent_attention: scale must be positive and in the range of 32 "
+                      "bits");
     for (const auto* x : {&lengths, &past}) {
         if (!x->has_value()) continue;
         TORCH_CHECK_TYPE((*x)->scalar_type() == torch::kInt,
@@ -451,7 +456,7 @@ torch::Tensor latent_attention_op(
         a.stats = reinterpret_cast<float2*>(stats.data_ptr<float>());
     }
     a.causal = causal;
-    a.scale = scale * 1.4426950408889634;
+    a.scale = scale2;
     if (dtype == torch::kBFloat16)
         latent_dispatch<__bf16>(a, nope, rope, blocks);
     else

@@ -31,6 +31,8 @@
 // tokens, fp16: 87 us, 640 TFLOP/s, and 12 us to join).
 #include <torch/extension.h>
 
+#include <cmath>
+
 #include <c10/core/DeviceGuard.h>
 
 #include "mfma_tiles.h"
@@ -737,8 +739,12 @@ torch::Tensor latent_cache_attention_op(
                       lengths.dim() == 1 && lengths.size(0) == B,
                       "latent_cache_attention: block_table must be [B, P] "
                       "and lengths [B]");
-    TORCH_CHECK_VALUE(scale > 0.0 && std::isfinite(scale),
-                      "latent_cache_attention: scale must be positive");
+    // the kernel's scale, in powers of two; zero or infinite in 32 bits it
+    // would turn hidden scores into NaN
+    const float scale2 = scale * 1.4426950408889634;
+    TORCH_CHECK_VALUE(scale2 > 0.0f && std::isnormal(scale2),
+                      "latent_cache_attention: scale must be positive and in the range of 32 "
+                      "bits");
     auto out = torch::empty({B, Sq, H, latent_dim}, q.options());
     if (out.numel() == 0) return out;
     const int64_t page = cache.size(1), width = block_table.size(1);
@@ -775,7 +781,7 @@ torch::Tensor latent_cache_attention_op(
     a.page_shift = (page & (page - 1)) == 0 ? __builtin_ctzl(page) : -1;
     a.B = B, a.H = H, a.Sq = Sq, a.table_width = width;
     a.rows = Sq * H;
-    a.scale = scale * 1.4426950408889634;
+    a.scale = scale2;
     const int block_rows = a.rows <= 16 ? 16 : a.rows <= 32 ? 32 : 64;
     a.row_groups = (a.rows + block_rows - 1) / block_rows;
     // LDS holds one block a CU; no more runs than there can be tiles

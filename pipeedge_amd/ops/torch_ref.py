@@ -240,6 +240,14 @@ def _softmax_seen(scores: Tensor, seen: Tensor) -> Tensor:
     return weight / total.masked_fill(total == 0.0, 1.0)
 
 
+def _check_scale(op: str, scale: float):
+    """A scale that 32 bits hold in powers of two, as the kernels take it."""
+    limits = torch.finfo(torch.float32)
+    if not limits.tiny <= scale * math.log2(math.e) <= limits.max:
+        raise ValueError(f"{op}: scale must be positive and in the range of "
+                         "32 bits")
+
+
 def check_latent_attention(q: Tensor, kv: Tensor, k_rope: Tensor,
                            scale: float, lengths: Optional[Tensor],
                            past: Optional[Tensor]):
@@ -265,8 +273,7 @@ def check_latent_attention(q: Tensor, kv: Tensor, k_rope: Tensor,
     if kv.shape[:3] != (b, sk, h) or k_rope.shape[:2] != (b, sk):
         raise ValueError(f"{op}: q {list(q.shape)}, kv {list(kv.shape)} and "
                          f"k_rope {list(k_rope.shape)} do not match")
-    if not 0.0 < scale < math.inf:
-        raise ValueError(f"{op}: scale must be positive")
+    _check_scale(op, scale)
     for t in (lengths, past):
         if t is None:
             continue
@@ -336,8 +343,7 @@ def check_latent_cache_attention(q: Tensor, cache: Tensor,
     if block_table.dim() != 2 or block_table.shape[0] != b \
             or lengths.shape != (b,):
         raise ValueError(f"{op}: block_table must be [B, P] and lengths [B]")
-    if not 0.0 < scale < math.inf:
-        raise ValueError(f"{op}: scale must be positive")
+    _check_scale(op, scale)
 
 
 def latent_cache_attention(q: Tensor, cache: Tensor, block_table: Tensor,

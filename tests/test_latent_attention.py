@@ -642,3 +642,26 @@ def test_cache_graph_and_repeats(h):
         graphs[0].replay()
         torch.cuda.synchronize()
         assert torch.equal(outs[0], want) and torch.equal(outs[1], want)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("scale", [1e-50, 1e-39, 2.5e38, 1e60, math.inf,
+                                   math.nan, 0.0, -1.0])
+def test_scales_outside_32_bits(device, scale):
+    """Scales that are zero, subnormal or infinite in 32 bits, where they
+    turned hidden scores into NaN; the next ones inside give what they give."""
+    q, kv, k_rope = make_expanded(1, 3, 3, 2, 64, 32, torch.bfloat16, device)
+    c, cache, table, n = make_cache([5], 2, 4, 256, 32, 16, torch.bfloat16,
+                                    device)
+    with pytest.raises(ValueError):
+        ops.latent_attention(q, kv, k_rope, causal=True, scale=scale)
+    with pytest.raises(ValueError):
+        ops.latent_cache_attention(c, cache, table, n, latent_dim=256,
+                                   scale=scale)
+    # all weights alike, in rows that see one, two and three keys
+    out = ops.latent_attention(q, kv, k_rope, causal=True, scale=1e-37)
+    check(out, *expanded_exact(q, kv, k_rope, 1e-37, True, None, None),
+          q.dtype)
+    out = ops.latent_cache_attention(c, cache, table, n, latent_dim=256,
+                                     scale=1e-37)
+    check(out, *cache_exact(c, cache, table, [5], 256, 1e-37), q.dtype)
