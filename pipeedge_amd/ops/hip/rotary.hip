@@ -40,7 +40,7 @@ struct RotaryArgs {
     int pairs, offset;          // rotated columns: offset .. offset + 2*pairs
     int rot_items, items;       // work items a head, in all
     int copy_lo;                // copied items below the rotated columns
-    int tokens_per_block;
+    int block0, tokens_per_block;
     unsigned items_magic;       // ceil(2^32 / items)
     float scale, sign;
 };
@@ -83,7 +83,7 @@ template <typename T, int VEC, bool INTERLEAVED, typename POS>
 __global__ __launch_bounds__(ROTARY_THREADS) void rotary_kernel(
         RotaryArgs a) {
     extern __shared__ float2 turns[];       // [tokens_per_block][pairs]
-    const int tok0 = blockIdx.x * a.tokens_per_block;
+    const int tok0 = (a.block0 + blockIdx.x) * a.tokens_per_block;
     const int toks = min(a.tokens_per_block, a.tokens - tok0);
 
     for (int i = threadIdx.x; i < toks * a.pairs; i += ROTARY_THREADS) {
@@ -281,16 +281,22 @@ bool rotary_overlap(const torch::Tensor& q, const torch::Tensor& k,
         width * size - 1, false, tries);
 }
 
+// A launch has less than 2^32 threads, so very many tokens take several.
 template <typename T, int VEC, bool INTERLEAVED>
-void rotary_launch(const RotaryArgs& a, bool wide, int blocks, size_t lds) {
-    if (wide)
-        hipLaunchKernelGGL((rotary_kernel<T, VEC, INTERLEAVED, int64_t>),
-                           dim3(blocks), dim3(ROTARY_THREADS), lds,
-                           pe_current_stream(), a);
-    else
-        hipLaunchKernelGGL((rotary_kernel<T, VEC, INTERLEAVED, int32_t>),
-                           dim3(blocks), dim3(ROTARY_THREADS), lds,
-                           pe_current_stream(), a);
+void rotary_launch(RotaryArgs a, bool wide, int blocks, size_t lds) {
+    constexpr int MOST = (int)((1L << 32) / ROTARY_THREADS) - 1;
+    for (long first = 0; first < blocks; first += MOST) {
+        a.block0 = first;
+        const dim3 grid(std::min(blocks - a.block0, MOST));
+        if (wide)
+            hipLaunchKernelGGL((rotary_kernel<T, VEC, INTERLEAVED, int64_t>),
+                               grid, dim3(ROTARY_THREADS), lds,
+                               pe_current_stream(), a);
+        else
+            hipLaunchKernelGGL((rotary_kernel<T, VEC, INTERLEAVED, int32_t>),
+                               grid, dim3(ROTARY_THREADS), lds,
+                               pe_current_stream(), a);
+    }
 }
 
 template <typename T, int WIDE>

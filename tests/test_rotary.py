@@ -411,3 +411,17 @@ def test_rotary_refuses_gradients_of_frequencies(device):
     with torch.no_grad():
         out = ops.rotary(q, pos, freqs)
     assert torch.equal(out, ops.rotary(q, pos, freqs.detach()))
+
+
+@pytest.mark.gpu
+def test_rotary_more_tokens_than_one_launch_has_blocks():
+    """2^24 blocks of 256 threads are one more than a launch takes."""
+    tokens, near = 2 ** 24 + 70, 2 ** 24
+    freqs = ops.rotary_frequencies(2, device="cuda")
+    pos = torch.arange(tokens, device="cuda", dtype=torch.int32)
+    q = torch.randn(1, 1, 770, device="cuda", dtype=torch.bfloat16)
+    out = ops.rotary(q.expand(tokens, 1, 770), pos, freqs)
+    for some in (slice(0, 70), slice(near - 70, tokens)):
+        want = ops.rotary(q.expand(pos[some].numel(), 1, 770),
+                          pos[some].clone(), freqs)
+        assert torch.equal(out[some], want)
