@@ -410,14 +410,15 @@ torch::Tensor latent_attention_op(
     if (Sk == 0) return out.zero_();
     TORCH_CHECK_VALUE(Sq < (1L << 30) && Sk < (1L << 30),
                       "latent_attention: too many tokens");
-    TORCH_CHECK_VALUE(kv.stride(1) < (1L << 24) &&
-                      k_rope.stride(1) < (1L << 24),
-                      "latent_attention: tokens more than 32 MiB apart");
     const int64_t row_blocks = (Sq + ROWS - 1) / ROWS;
     TORCH_CHECK_VALUE(B * H * row_blocks < (1L << 31),
                       "latent_attention: too many rows");
     const auto qa = latent_aligned(q), kva = latent_aligned(kv);
     const auto ra = latent_aligned(k_rope);
+    // of what the kernel reads, which may be a copy with other strides
+    TORCH_CHECK_VALUE(Sk == 1 || (kva.stride(1) < (1L << 24) &&
+                                  ra.stride(1) < (1L << 24)),
+                      "latent_attention: tokens 32 MiB or more apart");
     torch::Tensor len_c, past_c;
     LatentArgs a = {};
     a.q = qa.data_ptr();

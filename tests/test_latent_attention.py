@@ -315,6 +315,30 @@ def test_expanded_refuses_far_tokens():
 
 
 @pytest.mark.gpu
+def test_expanded_token_distance_is_that_of_the_copy():
+    """Values that have to be copied count with the copy's distance between
+    tokens, and a single token has none."""
+    heads = 2 ** 17
+    q = torch.randn(1, 1, 1, 96, device="cuda").bfloat16()
+    kv = torch.randn(1, 2, 1, 131, device="cuda").bfloat16()[..., 3:]
+    k_rope = torch.randn(1, 2, 32, device="cuda").bfloat16()
+    many = kv.expand(1, 2, heads, 128)
+    with pytest.raises(ValueError):
+        ops.latent_attention(q.expand(1, 1, heads, 96), many, k_rope)
+    half = ops.latent_attention(q.expand(1, 1, heads // 2, 96),
+                                many[:, :, :heads // 2], k_rope)
+    one = ops.latent_attention(q, kv, k_rope)
+    assert torch.equal(half, one.expand_as(half))
+    want = ops.latent_attention(q, kv[:, :1], k_rope[:, :1])
+    room = torch.zeros(1, 1, 2 ** 25, device="cuda", dtype=q.dtype)
+    far = room.as_strided((1, 1, 1, 128), (2 ** 25, 2 ** 24, 128, 1))
+    rope = room.as_strided((1, 1, 32), (2 ** 25, 2 ** 24, 1), 2 ** 23)
+    far.copy_(kv[:, :1])
+    rope.copy_(k_rope[:, :1])
+    assert torch.equal(ops.latent_attention(q, far, rope), want)
+
+
+@pytest.mark.gpu
 def test_expanded_shared_range_graphs():
     """The partial sums are a graph's own: two graphs and eager calls on
     another stream, in turn and at once."""
