@@ -411,7 +411,8 @@ torch::Tensor latent_attention_op(
     TORCH_CHECK_VALUE(Sq < (1L << 30) && Sk < (1L << 30),
                       "latent_attention: too many tokens");
     const int64_t row_blocks = (Sq + ROWS - 1) / ROWS;
-    TORCH_CHECK_VALUE(B * H * row_blocks < (1L << 31),
+    // a launch has less than 2^32 threads
+    TORCH_CHECK_VALUE(B * H * row_blocks < (1L << 24),
                       "latent_attention: too many rows");
     const auto qa = latent_aligned(q), kva = latent_aligned(kv);
     const auto ra = latent_aligned(k_rope);

@@ -315,6 +315,20 @@ def test_expanded_refuses_far_tokens():
 
 
 @pytest.mark.gpu
+def test_expanded_refuses_more_rows_than_a_launch_takes():
+    q, kv, k_rope = make_expanded(1, 1, 1, 1, 64, 32, torch.bfloat16, "cuda")
+    b, h = 2 ** 10, 2 ** 14
+    with pytest.raises(ValueError):
+        ops.latent_attention(q.expand(b, 1, h, 96), kv.expand(b, 1, h, 128),
+                             k_rope.expand(b, 1, 32))
+    b -= 1
+    out = ops.latent_attention(q.expand(b, 1, h, 96),
+                               kv.expand(b, 1, h, 128),
+                               k_rope.expand(b, 1, 32))
+    assert torch.equal(out, kv[..., 64:].expand_as(out))
+
+
+@pytest.mark.gpu
 def test_expanded_token_distance_is_that_of_the_copy():
     """Values that have to be copied count with the copy's distance between
     tokens, and a single token has none."""
