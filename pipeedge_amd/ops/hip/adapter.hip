@@ -962,10 +962,22 @@ torch::Tensor adapter_linear_op(
                       "adapter_linear: unknown activation");
     int64_t M = 1;
     for (const auto s : lead) M *= s;
-    TORCH_CHECK_VALUE(K > 0 && M < (1L << 31) && N < (1L << 31),
+    TORCH_CHECK_VALUE(K > 0 && K < (1L << 31) && M < (1L << 31) &&
+                      N < (1L << 31),
                       "adapter_linear: no inner columns, or too many rows");
     if (M == 0 || N == 0)
         return torch::empty(out_sizes, x.options());
+    const int rank_pad = r <= 32 ? 32 : (r + 63) / 64 * 64;
+    const bool any = n > 0 && r > 0;
+    // A launch has less than 2^32 threads: of the inner values a block for 64
+    // rows of a request, and those that pad; of few rows one for 16 columns.
+    const int64_t per = by_row ? 1 : M / x.size(0);
+    const int64_t tiles = per >= 64 ? (per + 63) / 64 * (M / per)
+                                    : (M + 63) / 64;
+    TORCH_CHECK_VALUE(
+        (!any || (tiles + 256) * (r <= 32 ? 256 : 512) < (1L << 32)) &&
+        (M > STEP_ROWS || (N + 15) / 16 * 64 * STEP_WAVES < (1L << 32)),
+        "adapter_linear: too many rows or columns");
 
     const auto x2d = adapter_dense(x.reshape({M, K}));
     const auto w = adapter_dense(weight);
@@ -985,8 +997,6 @@ torch::Tensor adapter_linear_op(
         t = adapter_dense(*t);
         return reinterpret_cast<const __bf16*>(t->data_ptr());
     };
-    const int rank_pad = r <= 32 ? 32 : (r + 63) / 64 * 64;
-    const bool any = n > 0 && r > 0;
     auto inner = torch::empty({any ? M : 0, rank_pad}, x.options());
     auto out = torch::empty(out_sizes, x.options());
     ProductArgs a = {};
@@ -1001,7 +1011,7 @@ torch::Tensor adapter_linear_op(
     a.ad.up = reinterpret_cast<const __bf16*>(
         pad_up ? up_padded.data_ptr() : up_c.data_ptr());
     a.ad.row_ids = ids_c.data_ptr<int>();
-    a.ad.rows_per_id = by_row ? 1 : M / x.size(0);
+    a.ad.rows_per_id = per;
     a.ad.n_adapters = any ? n : 0;      // without any, no id is inside
     a.ad.rank = up_rank, a.ad.rank_pad = rank_pad;
     if (any) {

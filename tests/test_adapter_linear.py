@@ -300,3 +300,16 @@ def test_adapter_streams(shape, rank):
         torch.cuda.synchronize()
         for out, ref in zip(outs, want):
             assert torch.equal(out, ref)
+
+
+@pytest.mark.gpu
+def test_adapter_refuses_more_than_a_launch_takes():
+    x, w, down, up = make((1,), 8, 8, 40, 1, "cuda")
+    ids = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for batch, length in ((2 ** 29, 1), (2 ** 22, 128), (2 ** 22, 65)):
+        with pytest.raises(ValueError):
+            ops.adapter_linear(x.expand(batch, length, 8), w, down, up,
+                               ids.expand(batch))
+    with pytest.raises(ValueError):
+        ops.adapter_linear(x, w[:1].expand(2 ** 27, 8), down,
+                           up[:, :1].expand(1, 2 ** 27, 8), ids)
