@@ -312,4 +312,4 @@ def test_adapter_refuses_more_than_a_launch_takes():
                                ids.expand(batch))
     with pytest.raises(ValueError):
         ops.adapter_linear(x, w[:1].expand(2 ** 27, 8), down,
-                           up[:, :1].expand(1, 2 ** 27, 8), ids)
+                           up[:, :1].expand(1, 2 ** 27, 40), ids)
