@@ -518,6 +518,7 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void adapter_product_kernel(
     constexpr int SLICE = (BN + BM) * BK;       // one buffer: [W | x] images
     constexpr int PR = 64 / CH;                 // rows a piece of 1 KiB
     constexpr int PIECES = (BN + BM) / PR / (WN * WM);
+    static_assert(BUFS == 2 || BUFS == 3, "slices that are waited for");
     typedef TileVec<__bf16>::v8 v8;
     __shared__ __attribute__((aligned(256))) __bf16 smem[BUFS * SLICE];
 
@@ -645,12 +646,9 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void adapter_product_kernel(
     };
     // Slice t has arrived for this wave, and its reads of the slice before
     // are done; behind the barrier that holds for all waves. LDS-DMA arrives
-    // in order, so the pieces of later slices may stay on their way.
+    // in order, so the pieces of the slice behind it may stay on their way.
     const auto arrive = [&](int t) {
-        if (BUFS == 4 && t + 2 < staged && fast(t + 2))
-            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"(2 * PIECES)
-                         : "memory");
-        else if (BUFS >= 3 && t + 1 < staged && fast(t + 1))
+        if (BUFS == 3 && t + 1 < staged && fast(t + 1))
             asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"(PIECES)
                          : "memory");
         else
@@ -739,8 +737,7 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void adapter_product_kernel(
     // columns of a row and all accesses to memory are 16 B a lane. Chunk c (4
     // columns) of row r lies at c ^ r: no conflict on either side.
     constexpr int LDS = BUFS * SLICE * 2;
-    constexpr int LEAST = (BN * BM * 4 + LDS - 1) / LDS;
-    constexpr int PASSES = LEAST == 3 ? 4 : LEAST;
+    constexpr int PASSES = (BN * BM * 4 + LDS - 1) / LDS;
     constexpr int MP = MI / PASSES, ROWS = 32 * MP * WM;
     static_assert(MI % PASSES == 0, "whole tiles a pass");
     constexpr int C4 = BN / 4, C8 = BN / 8;
