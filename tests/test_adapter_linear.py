@@ -313,3 +313,92 @@ def test_adapter_refuses_more_than_a_launch_takes():
     with pytest.raises(ValueError):
         ops.adapter_linear(x, w[:1].expand(2 ** 27, 8), down,
                            up[:, :1].expand(1, 2 ** 27, 40), ids)
+
+
+def kernels_of(rows, n, rank, per):
+    """The kernels that the rules on sizes choose: the product's tile as
+    columns by rows, and the inner values'."""
+    def blocks(wide, high):
+        return -(-n // wide) * -(-rows // high)
+    pad = 32 if rank <= 32 else -(-rank // 64) * 64
+    tile = "step" if rows <= 64 else \
+        (256, 256) if blocks(256, 256) >= 200 else \
+        (256, 128) if blocks(256, 128) >= 160 else \
+        (128, 128) if blocks(128, 128) >= 128 else (64, 64)
+    if rows * max(pad, 64) <= 512 * 64:
+        inner = "row"
+    elif rows * pad >= 2048 * 64 * (2 if rank <= 32 else 1):
+        inner = "lds32" if rank <= 32 else "lds64"
+    else:
+        inner = 16 if rank <= 16 else 32 if rank <= 32 else 64
+    return tile, inner
+
+
+VARIANTS = [
+    # batch, rows of each, K, N, rank: tile, inner
+    (19, 197, 72, 3500, 8, (256, 256), 16),
+    (4, 1031, 200, 3333, 40, (256, 256), "lds64"),
+    (42, 200, 136, 1801, 28, (256, 256), "lds32"),
+    (12, 197, 136, 2300, 70, (256, 128), "lds64"),
+    (9, 300, 68, 2050, 24, (256, 128), 32),
+    (8, 197, 200, 2300, 8, (128, 128), 16),
+    (7, 211, 72, 1537, 44, (128, 128), 64),
+    (5, 257, 331, 2001, 3, (128, 128), 16),
+    (8200, 1, 72, 270, 12, (128, 128), "lds32"),
+    (41, 201, 67, 45, 32, (64, 64), "lds32"),
+    (5, 100, 264, 310, 60, (64, 64), "row"),
+    (3, 300, 100, 200, 90, (64, 64), 64),
+    (3, 700, 40, 130, 200, (64, 64), "lds64"),
+]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("batch,length,k,n,rank,tile,inner", VARIANTS)
+def test_adapter_variants(device, batch, length, k, n, rank, tile, inner):
+    """Every tile of the product with every odd end: rows, columns, K, rank;
+    ids by item and mixed row by row."""
+    assert kernels_of(batch * length, n, rank, length) == (tile, inner)
+    count = 5
+    x, w, down, up = make((batch, length), k, n, rank, count, device)
+    bias = torch.randn(n).bfloat16().to(device)
+    res = torch.randn(batch, length, n).bfloat16().to(device)
+    scales = (torch.rand(count) + 0.5).to(device)
+    ids = (torch.arange(batch) * 3 % (count + 1) - 1).int().to(device)
+    args = (x, w, down, up, ids)
+    check(ops.adapter_linear(*args), *args)
+    kw = dict(bias=bias, act="gelu", residual=res, scales=scales)
+    check(ops.adapter_linear(*args, **kw), *args, **kw)
+    ids = (torch.arange(batch * length) * 7 % (count + 2) - 1).int()
+    args = args[:4] + (ids.reshape(batch, length).to(device),)
+    kw = dict(bias=bias, scales=scales)
+    check(ops.adapter_linear(*args, **kw), *args, **kw)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("batch,length,k,n,rank,tile,inner", VARIANTS)
+def test_adapter_variants_isolate(device, batch, length, k, n, rank, tile,
+                                  inner):
+    """Undefined values of one adapter, one scale and one row in each of
+    them, ids by item and mixed row by row: every other row is as
+    without them."""
+    count = 4
+    x, w, down, up = make((batch, length), k, n, rank, count, device)
+    scales = torch.ones(count, device=device)
+    by_item = (torch.arange(batch) % (count + 1) - 1).int()
+    by_row = (torch.arange(batch * length) * 3 % (count + 1) - 1).int()
+    for ids in (by_item, by_row.reshape(batch, length)):
+        row_ids = ids.reshape(batch, -1).expand(batch, length)
+        ids = ids.to(device)
+        want = ops.adapter_linear(x, w, down, up, ids, scales=scales)
+        x2, down2, up2, scales2 = (t.clone() for t in (x, down, up, scales))
+        down2[1, rank - 1, k - 1] = float("inf")
+        up2[1] = float("nan")
+        scales2[2] = float("nan")
+        x2[1, length // 2, k // 2] = float("nan")
+        out = ops.adapter_linear(x2, w, down2, up2, ids, scales=scales2)
+        clean = (row_ids != 1) & (row_ids != 2)
+        bad = ~clean
+        clean[1, length // 2] = False
+        bad[1, length // 2] = True
+        assert torch.equal(out[clean], want[clean])
+        assert out[bad].isnan().all()
