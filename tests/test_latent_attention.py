@@ -177,6 +177,26 @@ def test_expanded_padding_stays_zero(device, causal, sq, sk, length, past):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("b,sq,sk,h,parts", [
+    (3, 1100, 1100, 11, 1),          # 297 blocks of 128 queries
+    (5, 1027, 1027, 13, 1),          # 585
+    (2, 300, 300, 113, 1),           # 678
+    (3, 200, 2600, 11, 5),           # 66, the keys in 5 parts each
+])
+def test_expanded_causal_order_of_many_blocks(device, b, sq, sk, h, parts):
+    """Causal blocks are put in another order where an XCD has more than 32:
+    each of them has to be there once."""
+    blocks = b * h * -(-sq // 128)
+    assert parts == max(1, min(512 // blocks, -(-sk // 64) // 8))
+    assert blocks * parts > 256 and blocks * parts % 8 != 0
+    q, kv, k_rope = make_expanded(b, sq, sk, h, 64, 32, torch.bfloat16,
+                                  device)
+    out = ops.latent_attention(q, kv, k_rope, causal=True)
+    check(out, *expanded_exact(q, kv, k_rope, 96 ** -0.5, True, None, None),
+          torch.bfloat16)
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_expanded_strides(device):
     """Views: heads first, part of wider rows, misaligned storage."""
     dtype = torch.float16
@@ -449,6 +469,32 @@ def test_cache_matches_exact(device, dtype, latent, rope, page, sq, h,
     out = ops.latent_cache_attention(q, cache, table, n, latent_dim=latent,
                                      scale=0.07)
     assert out.shape == (len(lengths), sq, h, latent) and out.dtype == dtype
+    check(out, *cache_exact(q, cache, table, lengths, latent, 0.07), dtype)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("latent,rope,page", [
+    (512, 64, 64), (512, 64, 7), (512, 32, 64), (512, 32, 1),
+    (256, 64, 24), (256, 32, 16), (256, 32, 5),
+])
+@pytest.mark.parametrize("sq,h", [(1, 33), (3, 27), (2, 64)])
+def test_cache_of_room_for_long_runs(device, dtype, latent, rope, page, sq,
+                                     h):
+    """More than 32 rows and tables that could hold long caches: two waves a
+    row group, each with half of a tile's tokens, whatever the lengths."""
+    lengths = [1500, 0, 700, 33, 1, 64]
+    q, cache, table, n = make_cache(lengths, sq, h, latent, rope, page, dtype,
+                                    device)
+    groups = -(-sq * h // 64)
+    # 16 tiles of 64 tokens for each of the runs that the chip takes
+    room = 16 * (256 // groups) * 64
+    wide = -(-room // (page * len(lengths))) + 1
+    assert wide > table.shape[1]
+    table = torch.nn.functional.pad(table, (0, wide - table.shape[1]),
+                                    value=-12345)
+    out = ops.latent_cache_attention(q, cache, table, n, latent_dim=latent,
+                                     scale=0.07)
     check(out, *cache_exact(q, cache, table, lengths, latent, 0.07), dtype)
 
 
