@@ -244,7 +244,9 @@ def rotary_(q: Tensor, positions: Tensor, freqs: Tensor,
             offset: int = 0, inverse: bool = False, scale: float = 1.0):
     """``rotary`` in place, for views of a larger tensor: the first 2H of the
     3H heads of a packed qkv, the rotary columns of each head, rows of a
-    cache. ``q`` and ``k`` must not overlap. Returns its arguments."""
+    cache. The turned columns of two heads, of ``q``, of ``k`` or of both, must
+    not overlap. Five and more dimensions whose leading ones are not one in
+    memory take a launch for each of the first. Returns its arguments."""
     run = _hip.rotary if _use_hip(q) else torch_ref.rotary
     out = run(q, positions, freqs, k, interleaved, offset, inverse, scale,
               True)
@@ -269,8 +271,9 @@ def latent_attention(q: Tensor, kv: Tensor, k_rope: Tensor, *,
     (int32 [B]) the position of its first query, Sk - Sq if both are absent; a
     ``causal`` query sees no key behind its own position. Queries whose
     position is outside their sequence are padding and come back zero; keys
-    and values behind a sequence may hold anything. A non-finite value inside
-    a sequence also reaches the earlier queries of its tile."""
+    and values behind a sequence may hold anything. A value inside it that is
+    not finite may also reach queries that do not see it, whose zero weight it
+    is multiplied with; keys reach only queries that see them."""
     if scale is None:
         scale = 1.0 / math.sqrt(max(q.shape[-1], 1))
     run = _hip.latent_attention if _use_hip(q) else torch_ref.latent_attention
@@ -293,8 +296,10 @@ def latent_cache_attention(q: Tensor, cache: Tensor, block_table: Tensor,
     projection is applied afterwards. Query i sees tokens up to its own
     position, lengths - Sq + i; one before the start comes back zero, as does
     an empty sequence. Table entries behind a sequence are not read. A length
-    that the table cannot hold, or a page number that the cache does not have,
-    makes that sequence's outputs NaN. All heads and queries of a sequence
+    that the table cannot hold, or a page number that the cache (of one page
+    at least) does not have, makes that sequence's outputs NaN. A latent value
+    that is not finite may also reach the call's earlier queries, whose zero
+    weight it is multiplied with, but no other sequence. All heads and queries of a sequence
     share one pass over its tokens; a few queries at a time are what it is
     made for."""
     run = _hip.latent_cache_attention if _use_hip(q) \

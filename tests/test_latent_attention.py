@@ -197,6 +197,29 @@ def test_expanded_causal_order_of_many_blocks(device, b, sq, sk, h, parts):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("part,column", [("plain", 3), ("rope", 30)])
+def test_expanded_hidden_keys_not_finite(device, part, column):
+    """A key that is not finite reaches only the queries that see it. Others
+    keep their result but not its bits: 32 rows move the reference of their
+    softmax at the same time, and a weight 2^(score - reference) is rounded
+    differently for another reference, within the same half step."""
+    q, kv, k_rope = make_expanded(1, 200, 200, 2, 64, 32, torch.bfloat16,
+                                  device)
+    want = ops.latent_attention(q, kv, k_rope, causal=True)
+    exact = expanded_exact(q, kv, k_rope, 96 ** -0.5, True, None, None)
+    for value in (math.nan, math.inf):
+        keys, rope = kv.clone(), k_rope.clone()
+        (keys[0, 77, 1] if part == "plain" else rope[0, 77])[column] = value
+        out = ops.latent_attention(q, keys, rope, causal=True)
+        check(out[:, :77], *(x[:, :77] for x in exact), torch.bfloat16)
+        assert torch.equal(out[:, :64], want[:, :64])
+        if part == "plain":
+            assert torch.equal(out[:, :, 0], want[:, :, 0])
+        if math.isnan(value):
+            assert out[:, 77:, 1].isnan().all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_expanded_strides(device):
     """Views: heads first, part of wider rows, misaligned storage."""
     dtype = torch.float16
@@ -593,6 +616,34 @@ def test_cache_before_the_start_stays_zero(device, h, page):
         assert out[i, 303 - length:].any(-1).all()
         assert out[i, -1, :, 7].isnan().all() == (i < 2)
     assert out[2].isfinite().all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("h", [8, 16, 40])
+def test_cache_newest_row_not_finite(device, h):
+    """What the newest row holds reaches its own query and, where it is a
+    value, may reach earlier ones, but no other sequence; in the rotary
+    columns, which are keys alone, it reaches no earlier query. (The rows of a
+    wave move the reference of their softmax at the same time, so theirs may
+    be rounded differently, within the same half step.)"""
+    lengths = [70, 130, 5]
+    q, cache, table, n = make_cache(lengths, 2, h, 256, 32, 16,
+                                    torch.bfloat16, device)
+    kw = dict(latent_dim=256, scale=0.1)
+    want = ops.latent_cache_attention(q, cache, table, n, **kw)
+    ref = [x[1, 0] for x in cache_exact(q, cache, table, lengths, 256, 0.1)]
+    page, place = int(table[1, 129 // 16]), 129 % 16
+    for column in (9, 260):
+        for value in (math.nan, math.inf):
+            bad = cache.clone()
+            bad[page, place, column] = value
+            out = ops.latent_cache_attention(q, bad, table, n, **kw)
+            assert torch.equal(out[0], want[0])
+            assert torch.equal(out[2], want[2])
+            assert not out[1, 1].isfinite().all()
+            other = torch.arange(256) != column
+            check(out[1, 0].cpu()[:, other], ref[0][:, other],
+                  ref[1][:, other], ref[2], torch.bfloat16)
 
 
 @pytest.mark.parametrize("device", DEVICES)
