@@ -402,3 +402,39 @@ def test_adapter_variants_isolate(device, batch, length, k, n, rank, tile,
         bad[1, length // 2] = True
         assert torch.equal(out[clean], want[clean])
         assert out[bad].isnan().all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("rows", [16, 17, 32, 33, 64, 65, 129])
+@pytest.mark.parametrize("k,n,rank", [(1, 1, 1), (9, 7, 2), (40, 8, 8)])
+def test_adapter_smallest(device, rows, k, n, rank):
+    """One column, one rank, one K, at the numbers of rows where the kernels
+    change; items of more than one dimension."""
+    x, w, down, up = make((rows, 1, 2), k, n, rank, 3, device)
+    res = torch.randn(rows, 1, 2, n).bfloat16().to(device)
+    ids = (torch.arange(rows) % 4 - 1).int().to(device)
+    out = ops.adapter_linear(x, w, down, up, ids, act="tanh", residual=res)
+    check(out, x, w, down, up, ids, act="tanh", residual=res)
+    each = ids.reshape(rows, 1, 1).expand(rows, 1, 2)
+    assert torch.equal(ops.adapter_linear(x, w, down, up, each, act="tanh",
+                                          residual=res), out)
+    half = ops.adapter_linear(x[:, :, 0], w, down, up, ids)
+    check(half, x[:, :, 0], w, down, up, ids)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [4, 100, 3000])
+@pytest.mark.parametrize("rank", [64, 60])
+def test_adapter_far_stacks(rows, rank):
+    """Adapters behind 2^32 bytes of their stacks."""
+    k, n = 1032, 1096
+    count = 2 ** 31 // (n * rank) + 40
+    x, w, down, up = make((rows,), k, n, rank, 3, "cuda")
+    ids = (torch.arange(rows) % 4 - 1).int().cuda()
+    want = ops.adapter_linear(x, w, down, up, ids)
+    far_down = torch.empty(count, rank, k, dtype=x.dtype, device="cuda")
+    far_up = torch.empty(count, n, rank, dtype=x.dtype, device="cuda")
+    far_down[-3:], far_up[-3:] = down, up
+    assert far_up[-3].storage_offset() > 2 ** 31
+    far = torch.where(ids >= 0, ids + (count - 3), ids)
+    assert torch.equal(ops.adapter_linear(x, w, far_down, far_up, far), want)

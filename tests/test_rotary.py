@@ -425,3 +425,22 @@ def test_rotary_more_tokens_than_one_launch_has_blocks():
         want = ops.rotary(q.expand(pos[some].numel(), 1, 770),
                           pos[some].clone(), freqs)
         assert torch.equal(out[some], want)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dim,width,offset,h", [
+    (2048, 2048, 0, 3), (2050, 2048, 1, 1), (1600, 1040, 560, 2)])
+def test_rotary_wide_heads(device, interleaved, dim, width, offset, h):
+    """Up to the 2048 columns that are turned at most."""
+    torch.manual_seed(dim)
+    q = torch.randn(2, 5, h, dim, device=device).bfloat16()
+    pos = torch.randint(0, 9999, (2, 5), device=device)
+    freqs = ops.rotary_frequencies(width, device=device)
+    out = ops.rotary(q, pos, freqs, interleaved=interleaved, offset=offset)
+    check(out, q, pos, freqs, interleaved, offset, False, 1.0)
+    ops.rotary_(q, pos, freqs, interleaved=interleaved, offset=offset)
+    assert torch.equal(q, out)
+    with pytest.raises(ValueError):
+        ops.rotary(torch.zeros(1, 1, 2050, device=device), pos[0, :1],
+                   ops.rotary_frequencies(2050, device=device))
