@@ -5,10 +5,12 @@
 // activation, so y is written once and W is read as without adapters. The
 // inner values are rounded to bf16 once, as the operand of the second product;
 // the sums before and after stay in fp32. Few rows are bound by the latency of
-// two launches and of reading W (8 rows, 1024 to 4096 columns, rank 16: 9 to
-// 10 us), many by the product and by its epilogue, which nothing hides with one
-// block a CU (12608 rows, 1280 to 5120 columns, rank 64, gelu: 12 us and 240 to
-// 260, 640 TFLOP/s).
+// two launches and of reading W (8 rows, 1024 to 4096 columns, rank 16: 10 us),
+// many by the product and by its epilogue, which nothing hides with one block a
+// CU (12608 rows, 1280 to 5120 columns, rank 64, gelu: 12 us and 233, 710
+// TFLOP/s). Each further adapter among a tile's rows is a turn of its own in
+// both launches (4096 rows, 1280 to 1280, rank 64, ids mixed row by row: 28 us
+// without adapters, 36 with one, 88 with 8, 462 with 64).
 #include <torch/extension.h>
 
 #include <c10/core/DeviceGuard.h>
@@ -837,7 +839,10 @@ void adapter_inner(InnerArgs a) {
     // rows in turn. Whole projection, 1280 to 1280 columns, rank 64, us with
     // it and without, rows of one adapter and of 8 mixed: 256 rows 14 and 18,
     // 18 and 62; 512 rows 17 and 18, 21 and 63; 1024 rows 23 and 20, 28 and
-    // 71; 768 to 768, rank 8, 512 rows: 12 and 11, 15 and 22.
+    // 71; 768 to 768, rank 8, 512 rows: 12 and 11, 15 and 22. The rule is that
+    // of rows in order, by item; for rows of many adapters mixed one by one,
+    // which it does not tell apart, this kernel would be the better one far
+    // beyond 512.
     if ((long)a.M * std::max(a.rank_pad, 64) <= 512 * 64) {
         a.row_blocks = a.M;
         hipLaunchKernelGGL(adapter_inner_step_kernel,

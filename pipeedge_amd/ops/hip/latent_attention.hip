@@ -15,9 +15,9 @@
 // Bound by what a wave does in turn: 40 MFMAs a tile (1280 cycles of a SIMD),
 // then 32 exponentials a lane and their sums, with a second wave on the SIMD
 // to fill the gaps. 4099 queries against 8198 keys, 16 heads of 128 + 64, bf16
-// causal: 305 us, 850 TFLOP/s of about 1450 that a large matrix product
-// reaches (4096 tokens of 16 heads without a mask: 1030); without exponentials
-// 7% less, without loads 17% less time.
+// causal: 277 us (296 on the slowest card), 930 TFLOP/s of about 1450 that a
+// large matrix product reaches (4096 tokens of 16 heads without a mask: 1030);
+// without exponentials 7% less, without loads 17% less time.
 #include <torch/extension.h>
 
 #include <algorithm>

@@ -27,8 +27,11 @@
 // segment's end. Up to 16 rows a wave loads its own tokens, two tiles ahead,
 // and waits for nobody else. 16 heads are bound by memory (64 ragged sequences
 // up to 4096, 165 MB: 35 us, 4.7 TB/s, and 5 us to join), 128 heads by the
-// instructions around the MFMAs (2 queries of 16 sequences of 4096 to 8192
-// tokens, fp16: 87 us, 640 TFLOP/s, and 12 us to join).
+// instructions around the MFMAs and by the LDS, each fragment read from it
+// feeding one MFMA (2 queries of 16 sequences of 4096 to 8192 tokens, fp16: 84
+// us, 660 TFLOP/s, and 12 us to join). Two waves a SIMD with 512 columns are 15
+// registers short, which go to scratch memory, outside the loop over the
+// tiles.
 #include <torch/extension.h>
 
 #include <cmath>
